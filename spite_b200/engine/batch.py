@@ -36,6 +36,10 @@ class StepBatch:
     max_seg_len: int = 0
     context_bucket: int | None = None   # steps replayed from a CUDA graph: launch shapes are chosen for
                                         # this context length instead of the step's own
+    ancestors: torch.Tensor | None = None   # a step that verifies drafted tokens: [M, words] int32, bit a of row m: token m of its
+                                        # request descends from the request's token a (or is it); None: every token follows the one before
+    slot_maps: list | None = None       # per group: [M] int64, the cache row (page * page_size + offset) that a token's keys and
+                                        # values go to, -1: none; None: the row of the token's position
     shared: dict = field(default_factory=dict)   # what one layer of the step leaves for a later one (emptied when a
                                                  # forward pass starts)
 

@@ -63,6 +63,30 @@ class DistanceBias:
         return cls(table.to(torch.float32)[index].t().contiguous(), torch.tensor(runs, dtype=torch.int32, device=dev))
 
 
+@dataclass
+class PageTables:
+    """The pages that requests hold, on the device, changed in place by `layout_step`: a row of `tables` for every slot."""
+    tables: torch.Tensor         # [rows, W] int32: page of a logical page (position // page_size); -1 in front of a row's first page and behind its last
+    held: torch.Tensor           # [rows] int32: logical pages that a row reaches to
+    page_size: int
+    window: object               # a `cache.Window`: which pages no later token reads
+    free_pages: Optional[torch.Tensor] = None    # [pages] int32: a stack of free pages; without one the tables must cover every token already
+    n_free: Optional[torch.Tensor] = None        # [1] int32: its height
+
+
+@dataclass
+class StepLayout:
+    """The integer inputs of a step of S requests and up to M tokens, as `layout_step` writes them."""
+    OUT_OF_PAGES, MALFORMED = 1, 2               # bits of `status`
+    block_table: torch.Tensor    # [S, W'] int32
+    cu_seqlens: torch.Tensor     # [S + 1] int32
+    positions: torch.Tensor      # [M] int32; here and below: rows behind the last request's token are left as they were
+    seg_of_token: torch.Tensor   # [M] int32
+    slot_map: torch.Tensor       # [M] int64: page * page_size + offset of the token's row of the cache, -1: none
+    status: torch.Tensor         # [1] int32: 0, or why the step was not laid out
+    ancestors: Optional[torch.Tensor] = None     # [M, words] int32: bit a of row m: token m of its request descends from the request's token a, or is it
+
+
 class KernelSet:
     """Interface; see `CudaKernels` for the product implementation.
 
@@ -258,6 +282,43 @@ class KernelSet:
         `cache_settled`: the caller promises that the cache rows of positions before each request's first
         token of this step were written by earlier steps (not by the one or two kernels launched just
         before this call), so a kernel may fetch them while the kernel before still runs."""
+        raise NotImplementedError
+
+    def tree_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, sink_logit=None, head_sinks=None, head_slopes=None,
+                       head_gates=None, out_by_head=False, score_softcap=None, distance_bias=None):
+        """`paged_attention` for a step whose requests bring trees of drafted tokens (up to 1024 a request): `batch.ancestors` [M, words]
+        int32.  A request with n tokens and len cached ones keeps node i's key at place len + i, while node i's position
+        (`batch.positions`) is len + its depth; node 0 has depth 0.  Node i sees the places below len that `window` lets its position see, and of
+        the nodes up to itself those whose bit is set in its row and in their own (a node without its own bit is padding: nobody sees
+        it, and its row of the cache may hold anything, as may the rows behind the last node), unless its window ends behind
+        their position.  Distances are between positions.  A row that sees nothing is zero.  Everything else as in `paged_attention`;
+        `batch` needs positions, seg_of_token, cu_seqlens, block_tables and ancestors, and the host need not know how much is cached.  Rows of
+        `out` behind the last request's are left as they were."""
+        raise NotImplementedError
+
+    # ---- steps laid out and drafts accepted on the device
+    def layout_step(self, pages, slots, lengths, new_tokens, out, *, parents=None):
+        """The integer inputs of a step from the requests' lengths, without the host.  Request s stands in row slots[s] (int32 [S], each row
+        once; -1: padding, no tokens) of `pages` (`PageTables`) and of `lengths` (int32 [rows], tokens cached), and brings new_tokens[s]
+        (int32) tokens; -1: it has ended.  First the pages that no later token's window reaches (all of an ended request) go back on the
+        stack, in the order of s and ascending; then the pages that the step's tokens need come off its top, in the same order.  `out`
+        (`StepLayout`): block_table[s] is the request's row (-1 for ended ones and padding), positions[m] = lengths + number within the request, or with
+        `parents` (int32, per token of the step: the number within the request of its parent, which is smaller; -1: none; below: padding) +
+        depth in the tree; slot_map[m] the cache row of place lengths + number (-1 for padding); ancestors as `tree_attention` reads them.  A token
+        whose parent is not smaller has none.  With `parents` or `ancestors` a request brings up to 1024 tokens.
+        What only the device can see is said in out.status: `StepLayout.OUT_OF_PAGES`, or MALFORMED (a slot twice or outside the tables, a
+        length that the row does not cover, more tokens or pages than `out` has room for); then nothing of `pages` has changed, block_table is -1
+        and the step has no tokens.  `lengths` stays as it is.  Calling it again with the same lengths takes no further pages."""
+        raise NotImplementedError
+
+    def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
+        """Follows every request's tree (tokens, parents as in `layout_step`, None: chains; int32 [M]) by what the model says: from node 0 to the
+        lowest-numbered child that is the node's target (targets, int32 [M]), and on.  counts [S] int32: nodes on the way (0 for a request without
+        tokens), path [S, D] int32 their numbers, emitted [S, D] their targets, -1 behind the last; a way ends after D nodes.  The rows
+        of the way's nodes move to the places that follow the request's cached tokens: in every cache of `caches`, a list of (kv [caches, planes,
+        pages, kv heads, page_size, head_dim], slot_map [M] int64, key_scales [caches, pages, kv heads, page_size] float32 or None), the row of
+        slot_map[node] goes to slot_map[number on the way] (no row where either is negative).  With `lengths` (int32 [rows], and `lengths_out`, which may
+        be the same): lengths_out[slots[s]] = lengths[slots[s]] + counts[s] (without `slots`: row s)."""
         raise NotImplementedError
 
     # ---- attention through latents

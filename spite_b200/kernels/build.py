@@ -38,6 +38,8 @@ LIBRARIES = {
     "attention_decode": (["attention_decode.cu"], []),
     "attention_rows": (["attention_rows.cu"], []),
     "attention_tc": (["attention_tc.cu"], []),
+    "attention_tree": (["attention_tree.cu"], []),
+    "drafts": (["drafts.cu"], []),
     "moe": (["moe.cu"], []),
     "latent": (["latent.cu"], []),
     "recurrent": (["recurrent.cu"], []),

@@ -144,6 +144,35 @@ class AttnDecodeExtra(C.Structure):
                 ("seg_min_tokens", C.c_int), ("seg_max_tokens", C.c_int), ("cache_settled", C.c_int)]
 
 
+class TreeStep(C.Structure):
+    _fields_ = [("cu_seqlens", C.c_void_p), ("ancestors", C.c_void_p), ("n_segments", C.c_int), ("n_words", C.c_int)]
+
+
+class LayoutParams(C.Structure):
+    _fields_ = [("tables", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p), ("n_free", C.c_void_p),
+                ("slots", C.c_void_p), ("lengths", C.c_void_p), ("new_tokens", C.c_void_p), ("parents", C.c_void_p),
+                ("block_table", C.c_void_p), ("cu_seqlens", C.c_void_p), ("positions", C.c_void_p), ("seg_of_token", C.c_void_p),
+                ("slot_map", C.c_void_p), ("ancestors", C.c_void_p), ("status", C.c_void_p),
+                ("n_rows", C.c_int), ("table_width", C.c_int), ("n_pages", C.c_int), ("n_requests", C.c_int), ("out_width", C.c_int),
+                ("n_tokens", C.c_int), ("n_parents", C.c_int), ("n_words", C.c_int), ("page_size", C.c_int), ("window_kind", C.c_int),
+                ("window_size", C.c_int)]
+
+
+class AcceptGroup(C.Structure):
+    _fields_ = [("kv", C.c_void_p), ("key_scales", C.c_void_p), ("slot_map", C.c_void_p), ("plane_bytes", C.c_longlong),
+                ("planes", C.c_int), ("caches", C.c_int), ("n_pages", C.c_int), ("num_kv_heads", C.c_int), ("page_size", C.c_int),
+                ("row_bytes", C.c_int)]
+
+
+class AcceptParams(C.Structure):
+    MAX_GROUPS = 8
+    _fields_ = [("tokens", C.c_void_p), ("parents", C.c_void_p), ("targets", C.c_void_p), ("cu_seqlens", C.c_void_p),
+                ("counts", C.c_void_p), ("path", C.c_void_p), ("emitted", C.c_void_p), ("slots", C.c_void_p),
+                ("lengths", C.c_void_p), ("lengths_out", C.c_void_p),
+                ("n_tokens", C.c_int), ("n_requests", C.c_int), ("depth", C.c_int), ("n_rows", C.c_int), ("n_groups", C.c_int),
+                ("groups", AcceptGroup * MAX_GROUPS)]
+
+
 class SampleParams(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("work", C.c_void_p), ("temperature", C.c_void_p),
                 ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
@@ -1069,25 +1098,24 @@ class CudaKernels(KernelSet):
         self._count("attention", 1)
         _check(st, "turn_heads")
 
-    def paged_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, cache_settled=False,
-                        sink_logit=None, head_sinks=None, head_slopes=None, head_gates=None, out_by_head=False,
-                        score_softcap=None, distance_bias=None):
+    def _attention_params(self, what, q, out, num_heads, window, softmax_scale, sink_logit, head_sinks, head_slopes, head_gates, out_by_head,
+                          score_softcap, distance_bias):
         self._t(q, self.dtype, "q"); self._t(out, self.dtype, "out")
         if score_softcap is not None and not score_softcap > 0:
-            raise KernelError("paged_attention: the cap of the scores must be positive")
+            raise KernelError(f"{what}: the cap of the scores must be positive")
         if out.numel() != q.numel():
-            raise KernelError("paged_attention: out must have as many elements as q")
+            raise KernelError(f"{what}: out must have as many elements as q")
         for name, t, n in (("head_sinks", head_sinks, num_heads), ("head_slopes", head_slopes, num_heads),
                            ("head_gates", head_gates, q.shape[0] * num_heads)):
             if t is not None and self._t(t, torch.float32, name).numel() != n:
-                raise KernelError(f"paged_attention: {name} has {t.numel()} elements, {n} are needed")
+                raise KernelError(f"{what}: {name} has {t.numel()} elements, {n} are needed")
         if not softmax_scale > 0:
-            raise KernelError("paged_attention: the score scale must be positive")
+            raise KernelError(f"{what}: the score scale must be positive")
         if distance_bias is not None:
             self._t(distance_bias.runs, torch.int32, "distance_bias.runs")
             if tuple(self._t(distance_bias.padded, torch.float32, "distance_bias.padded").shape) != \
                     (num_heads, distance_bias.length + 2 * distance_bias.PAD):
-                raise KernelError("paged_attention: one row of numbers by distance per head")
+                raise KernelError(f"{what}: one row of numbers by distance per head")
         p = AttentionParams(q=q.data_ptr(), out=out.data_ptr(), num_heads=num_heads,
                             window_kind=_WINDOW[window.kind], window_size=int(window.size),
                             softmax_scale=float(softmax_scale),
@@ -1098,6 +1126,13 @@ class CudaKernels(KernelSet):
         if distance_bias is not None:
             p.distance_bias, p.distance_runs = distance_bias.padded.data_ptr(), distance_bias.runs.data_ptr()
             p.distance_len = distance_bias.length
+        return p
+
+    def paged_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, cache_settled=False,
+                        sink_logit=None, head_sinks=None, head_slopes=None, head_gates=None, out_by_head=False,
+                        score_softcap=None, distance_bias=None):
+        p = self._attention_params("paged_attention", q, out, num_heads, window, softmax_scale, sink_logit, head_sinks, head_slopes, head_gates,
+                                   out_by_head, score_softcap, distance_bias)
         b, c = self._step_tokens(batch, cache.group), self._paged(cache)
         group = num_heads // c.num_kv_heads
         if (self.dtype == torch.bfloat16 and c.head_dim % 16 == 0 and c.head_dim <= 128 and group <= 16
@@ -1225,6 +1260,132 @@ class CudaKernels(KernelSet):
             C.byref(p), C.byref(b), C.byref(c), C.byref(x), n_small, n_stages, self._stream())
         self._count("attention_decode", 1)
         _check(st, "paged_attention (decode)")
+
+    def tree_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, sink_logit=None, head_sinks=None, head_slopes=None,
+                       head_gates=None, out_by_head=False, score_softcap=None, distance_bias=None):
+        p = self._attention_params("tree_attention", q, out, num_heads, window, softmax_scale, sink_logit, head_sinks, head_slopes, head_gates,
+                                   out_by_head, score_softcap, distance_bias)
+        M, table = batch.n_tokens, batch.block_tables[cache.group]
+        S = batch.cu_seqlens.numel() - 1
+        if batch.ancestors is None:
+            raise KernelError("tree_attention: the step has no ancestor sets")
+        for name, t, size in (("positions", batch.positions, M), ("seg_of_token", batch.seg_of_token, M), ("cu_seqlens", batch.cu_seqlens, 2),
+                              ("block_table", table, S), ("ancestors", batch.ancestors, M)):
+            if self._t(t, torch.int32, name).numel() < size:
+                raise KernelError(f"tree_attention: {name} has {t.numel()} elements for {M} tokens of {S} requests")
+        if table.dim() != 2 or table.shape[0] < S or batch.ancestors.dim() != 2 or batch.ancestors.shape[0] < M or not batch.ancestors.shape[1]:
+            raise KernelError("tree_attention: block_table is [requests, pages], ancestors [tokens, words]")
+        b, c = self._step_tokens(batch, cache.group), self._paged(cache)
+        if q.shape[0] != M or q.numel() != M * num_heads * c.head_dim or num_heads % c.num_kv_heads:
+            raise KernelError(f"tree_attention: q {tuple(q.shape)} does not hold {M} tokens of {num_heads} heads of {c.head_dim} ({c.num_kv_heads} kv heads)")
+        if c.head_dim > 256:
+            raise KernelError(f"tree_attention: heads of {c.head_dim} elements; up to 256 are supported")
+        if not M:
+            return
+        x = TreeStep(cu_seqlens=batch.cu_seqlens.data_ptr(), ancestors=batch.ancestors.data_ptr(), n_segments=S, n_words=batch.ancestors.shape[1])
+        # The multiply-add kernel: shares of the keys so that about eight blocks a multiprocessor run, none shorter than four tiles
+        # of 32 keys if the table is full.
+        group = num_heads // c.num_kv_heads
+        blocks = max(1, -(-M * min(group, 16) // 16)) * -(-group // 16) * c.num_kv_heads
+        keys = min(table.shape[1] * c.page_size, batch.context_bucket or (1 << 30))
+        if window.kind != "full":
+            keys = min(keys, window.size + 32 * x.n_words)
+        splits = max(1, min(32, 8 * self.sm_count // blocks, keys // 128))
+        part = torch.empty(M * num_heads * splits * (c.head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        st = self._lib("attention_tree").spite_tree_attention(self._dt, C.byref(p), C.byref(b), C.byref(c), C.byref(x), C.c_void_p(_ptr(part)),
+                                                              C.c_longlong(0 if part is None else part.numel()), splits, self._stream())
+        self._count("attention_tree", 1 + (splits > 1))
+        _check(st, "tree_attention")
+
+    # ------------------------------------------------------------------ steps laid out and drafts accepted on the device
+    def _ints(self, what, dtype=torch.int32, **tensors):
+        """The tensors named, checked to be contiguous whole numbers on the device with the number of dimensions given: name=(tensor, dimensions)."""
+        for name, (t, dims) in tensors.items():
+            if self._t(t, dtype, f"{what}: {name}").dim() != dims:
+                raise KernelError(f"{what}: {name} has {t.dim()} dimensions, {dims} are needed")
+
+    def layout_step(self, pages, slots, lengths, new_tokens, out, *, parents=None):
+        what = "layout_step"
+        self._ints(what, tables=(pages.tables, 2), held=(pages.held, 1), slots=(slots, 1), lengths=(lengths, 1), new_tokens=(new_tokens, 1),
+                   block_table=(out.block_table, 2), cu_seqlens=(out.cu_seqlens, 1), positions=(out.positions, 1),
+                   seg_of_token=(out.seg_of_token, 1), status=(out.status, 1))
+        self._ints(what, torch.int64, slot_map=(out.slot_map, 1))
+        if (pages.free_pages is None) != (pages.n_free is None):
+            raise KernelError(f"{what}: a stack of free pages needs its height, and the other way round")
+        if pages.free_pages is not None:
+            self._ints(what, free_pages=(pages.free_pages, 1), n_free=(pages.n_free, 1))
+        if parents is not None:
+            self._ints(what, parents=(parents, 1))
+        if out.ancestors is not None:
+            self._ints(what, ancestors=(out.ancestors, 2))
+        S, (R, W), M = slots.numel(), pages.tables.shape, out.positions.numel()
+        if pages.held.numel() != R or lengths.numel() != R or new_tokens.numel() != S or out.block_table.shape[0] != S or out.cu_seqlens.numel() != S + 1:
+            raise KernelError(f"{what}: {S} requests in {R} rows: held and lengths have a number a row, new_tokens and block_table one a request, cu_seqlens one more")
+        if out.seg_of_token.numel() != M or out.slot_map.numel() != M or (out.ancestors is not None and out.ancestors.shape[0] != M):
+            raise KernelError(f"{what}: positions, seg_of_token, slot_map and ancestors have room for the same number of tokens")
+        if out.status.numel() != 1 or (pages.n_free is not None and pages.n_free.numel() != 1):
+            raise KernelError(f"{what}: status and n_free are one number each")
+        if int(pages.page_size) < 1 or not W or not out.block_table.shape[1] or (out.ancestors is not None and not out.ancestors.shape[1]):
+            raise KernelError(f"{what}: empty pages, tables or sets")
+        if not S:
+            raise KernelError(f"{what}: a step needs a request")
+        plan = torch.empty(S, dtype=torch.int32, device=slots.device)
+        p = LayoutParams(tables=pages.tables.data_ptr(), held=pages.held.data_ptr(), free_pages=_ptr(pages.free_pages), n_free=_ptr(pages.n_free),
+                         slots=slots.data_ptr(), lengths=lengths.data_ptr(), new_tokens=new_tokens.data_ptr(), parents=_ptr(parents),
+                         block_table=out.block_table.data_ptr(), cu_seqlens=out.cu_seqlens.data_ptr(), positions=out.positions.data_ptr(),
+                         seg_of_token=out.seg_of_token.data_ptr(), slot_map=out.slot_map.data_ptr(), ancestors=_ptr(out.ancestors),
+                         status=out.status.data_ptr(), n_rows=R, table_width=W, n_pages=0 if pages.free_pages is None else pages.free_pages.numel(),
+                         n_requests=S, out_width=out.block_table.shape[1], n_tokens=M, n_parents=0 if parents is None else parents.numel(),
+                         n_words=0 if out.ancestors is None else out.ancestors.shape[1], page_size=int(pages.page_size),
+                         window_kind=_WINDOW[pages.window.kind], window_size=int(pages.window.size))
+        st = self._lib("drafts").spite_layout_step(C.byref(p), C.c_void_p(plan.data_ptr()), self._stream())
+        self._count("drafts", 2)
+        _check(st, what)
+
+    def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
+        what = "accept_drafts"
+        self._ints(what, tokens=(tokens, 1), targets=(targets, 1), cu_seqlens=(cu_seqlens, 1), counts=(counts, 1), path=(path, 2), emitted=(emitted, 2))
+        S, M = cu_seqlens.numel() - 1, tokens.numel()
+        if parents is not None:
+            self._ints(what, parents=(parents, 1))
+        if targets.numel() != M or (parents is not None and parents.numel() != M):
+            raise KernelError(f"{what}: {M} tokens have a parent and a target each")
+        if S < 1 or counts.numel() != S or path.shape != emitted.shape or path.shape[0] != S or not path.shape[1]:
+            raise KernelError(f"{what}: {S} requests: counts has a number, path and emitted a row of the same length for each")
+        if (lengths is None) != (lengths_out is None):
+            raise KernelError(f"{what}: lengths and lengths_out go together")
+        if slots is not None:
+            self._ints(what, slots=(slots, 1))
+            if slots.numel() != S:
+                raise KernelError(f"{what}: {slots.numel()} slots for {S} requests")
+        if lengths is not None:
+            self._ints(what, lengths=(lengths, 1), lengths_out=(lengths_out, 1))
+            if lengths.numel() != lengths_out.numel() or (slots is None and lengths.numel() < S):
+                raise KernelError(f"{what}: lengths and lengths_out have a number a row")
+        if len(caches) > AcceptParams.MAX_GROUPS:
+            raise KernelError(f"{what}: {len(caches)} groups of caches; up to {AcceptParams.MAX_GROUPS} in one call")
+        p = AcceptParams(tokens=tokens.data_ptr(), parents=_ptr(parents), targets=targets.data_ptr(), cu_seqlens=cu_seqlens.data_ptr(),
+                         counts=counts.data_ptr(), path=path.data_ptr(), emitted=emitted.data_ptr(), slots=_ptr(slots), lengths=_ptr(lengths),
+                         lengths_out=_ptr(lengths_out), n_tokens=M, n_requests=S, depth=path.shape[1],
+                         n_rows=0 if lengths is None else lengths.numel(), n_groups=len(caches))
+        most = 1
+        for g, (kv, slot_map, scales) in enumerate(caches):
+            if self._t(kv, self.dtype, f"{what}: cache").dim() != 6 or not kv.numel():
+                raise KernelError(f"{what}: a cache is [caches, planes, pages, kv heads, page_size, head_dim]")
+            self._ints(what, torch.int64, slot_map=(slot_map, 1))
+            if slot_map.numel() < M:
+                raise KernelError(f"{what}: the slot map has {slot_map.numel()} rows for {M} tokens")
+            n, planes, n_pages, heads, page_size, size = kv.shape
+            if scales is not None and tuple(self._t(scales, torch.float32, f"{what}: key_scales").shape) != (n, n_pages, heads, page_size):
+                raise KernelError(f"{what}: key_scales are [caches, pages, kv heads, page_size]")
+            p.groups[g] = AcceptGroup(kv=kv.data_ptr(), key_scales=_ptr(scales), slot_map=slot_map.data_ptr(), plane_bytes=kv.stride(1) * kv.element_size(),
+                                      planes=n * planes, caches=n, n_pages=n_pages, num_kv_heads=heads, page_size=page_size, row_bytes=size * kv.element_size())
+            most = max(most, n * planes * heads * size * kv.element_size() // 16)
+        # a thread for every 16 bytes of a token's rows, as long as that is not far more blocks than the device holds
+        pieces = max(1, min(-(-most // 256), max(1, 16 * self.sm_count // S)))
+        st = self._lib("drafts").spite_accept_drafts(C.byref(p), pieces, self._stream())
+        self._count("drafts", 1)
+        _check(st, what)
 
     # ------------------------------------------------------------------ attention through latents
     def latent_prepare(self, down, cq_out, batch, cache, *, q_rank, kv_rank, rotation, q_gain, kv_gain, eps,
