@@ -39,6 +39,7 @@ LIBRARIES = {
     "attention_rows": (["attention_rows.cu"], []),
     "attention_tc": (["attention_tc.cu"], []),
     "attention_tree": (["attention_tree.cu"], []),
+    "attention_tree_tc": (["attention_tree_tc.cu"], []),
     "drafts": (["drafts.cu"], []),
     "moe": (["moe.cu"], []),
     "latent": (["latent.cu"], []),

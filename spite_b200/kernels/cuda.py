@@ -185,7 +185,7 @@ class SampleParams(C.Structure):
 # library's word of one small buffer in pinned host memory, which the device writes directly: the host
 # reads it after any point at which it has waited for a step's results, without another copy or wait.
 _WAITING_LIBRARIES = ("gemm_tc", "gemm_tc_pair", "gemm_stream", "attention_tc", "attention_decode", "gemm_tc_experts", "delta",
-                      "recurrent", "scan")
+                      "recurrent", "scan", "attention_tree_tc")
 _error_words = None          # pinned int32 [len(_WAITING_LIBRARIES)], one per process
 _configured: set = set()
 
@@ -1283,6 +1283,16 @@ class CudaKernels(KernelSet):
         if not M:
             return
         x = TreeStep(cu_seqlens=batch.cu_seqlens.data_ptr(), ancestors=batch.ancestors.data_ptr(), n_segments=S, n_words=batch.ancestors.shape[1])
+        if (self.dtype == torch.bfloat16 and c.head_dim in (64, 128) and c.page_size % 64 == 0 and self.use_tcgen05_attention
+                and distance_bias is None and cache.kv.shape[0] == 2 and cache.key_scale is None):
+            n_floats = self.sm_count * (4 * (c.head_dim + 2) * 128 + 8)
+            part = torch.empty(n_floats, dtype=torch.float32, device=q.device)
+            st = self._lib("attention_tree_tc").spite_tree_attention_tc(C.byref(p), C.byref(b), C.byref(c), C.byref(x), self.sm_count, C.c_void_p(part.data_ptr()),
+                                                                        C.c_longlong(n_floats), self._stream())
+            if st != -2:                        # -2: more than 128 heads a kv head, 2,048 requests, a row that does not start at 16 bytes
+                self._count("attention_tree_tc", 2)
+                _check(st, "tree_attention (tcgen05)")
+                return
         # The multiply-add kernel: shares of the keys so that about eight blocks a multiprocessor run, none shorter than four tiles
         # of 32 keys if the table is full.
         group = num_heads // c.num_kv_heads
