@@ -257,18 +257,14 @@ int launch(const AttentionParams& p, const StepTokens& b, const PagedCache& c, c
 }  // namespace
 
 // `partial`: tokens * heads * n_splits * (head_dim + 2) floats where n_splits (1..32) > 1.
-SPITE_API int spite_tree_attention(int dtype, const AttentionParams* p, const StepTokens* b, const PagedCache* c, const TreeStep* x, float* partial,
-                                   long long n_partial, int n_splits, void* stream) {
-    if (!p || !b || !c || !x || !p->q || !p->out || !c->kv || !b->positions || !b->seg_of_token || !b->block_table || !x->cu_seqlens || !x->ancestors)
-        return SPITE_BAD_ARG;
-    if (b->n_tokens < 0 || b->table_width < 1 || c->n_pages < 1 || c->page_size < 1 || x->n_segments < 1 || x->n_words < 1) return SPITE_BAD_ARG;
-    if (p->num_heads < 1 || c->num_kv_heads < 1 || p->num_heads % c->num_kv_heads || c->head_dim < 1) return SPITE_BAD_ARG;
-    if (p->window_kind < 0 || p->window_kind > 2 || (p->window_kind != SPITE_WINDOW_FULL && p->window_size < 1) || !distance_bias_ok(p)) return SPITE_BAD_ARG;
-    if (n_splits < 1 || n_splits > 32 || (n_splits > 1 && (!partial || n_partial < (long long)b->n_tokens * p->num_heads * n_splits * (c->head_dim + 2))))
-        return SPITE_BAD_ARG;
-    if (c->head_dim > 256 || p->num_heads > 4 * 65535) return SPITE_UNSUPPORTED;
-    if (b->n_tokens == 0) return SPITE_OK;
-    if (dtype == SPITE_DT_F32) return launch<float>(*p, *b, *c, *x, partial, n_splits, (cudaStream_t)stream);
-    if (dtype == SPITE_DT_BF16) return launch<__nv_bfloat16>(*p, *b, *c, *x, partial, n_splits, (cudaStream_t)stream);
+SPITE_API int spite_tree_attention(int dtype, const TreeCall* call, float* partial, long long n_partial, int n_splits, void* stream) {
+    if (!call || !tree_call_ok(*call)) return SPITE_BAD_ARG;
+    const AttentionParams& p = call->p;
+    if (n_splits < 1 || n_splits > 32) return SPITE_BAD_ARG;
+    if (n_splits > 1 && (!partial || n_partial < (long long)call->b.n_tokens * p.num_heads * n_splits * (call->c.head_dim + 2))) return SPITE_BAD_ARG;
+    if (call->c.head_dim > 256 || p.num_heads > 4 * 65535) return SPITE_UNSUPPORTED;
+    if (call->b.n_tokens == 0) return SPITE_OK;
+    if (dtype == SPITE_DT_F32) return launch<float>(p, call->b, call->c, call->x, partial, n_splits, (cudaStream_t)stream);
+    if (dtype == SPITE_DT_BF16) return launch<__nv_bfloat16>(p, call->b, call->c, call->x, partial, n_splits, (cudaStream_t)stream);
     return SPITE_BAD_ARG;
 }

@@ -15,6 +15,20 @@ struct TreeStep {
     int n_words;
 };
 
+// What a call is given.
+struct TreeCall {
+    AttentionParams p;
+    StepTokens b;
+    PagedCache c;
+    TreeStep x;
+};
+static inline bool tree_call_ok(const TreeCall& a) {
+    if (!a.p.q || !a.p.out || !a.c.kv || !a.b.positions || !a.b.seg_of_token || !a.b.block_table || !a.x.cu_seqlens || !a.x.ancestors) return false;
+    if (a.b.n_tokens < 0 || a.b.table_width < 1 || a.c.n_pages < 1 || a.c.page_size < 1 || a.x.n_segments < 1 || a.x.n_words < 1) return false;
+    if (a.p.num_heads < 1 || a.c.num_kv_heads < 1 || a.p.num_heads % a.c.num_kv_heads || a.c.head_dim < 1) return false;
+    return a.p.window_kind >= 0 && a.p.window_kind <= 2 && (a.p.window_kind == SPITE_WINDOW_FULL || a.p.window_size >= 1) && distance_bias_ok(&a.p);
+}
+
 // Is node `i` of the segment that starts at token `first` a token of its own (its own bit is set)?
 __device__ __forceinline__ bool tree_node_is_real(const TreeStep& x, int first, int i) {
     return i < 32 * x.n_words && (x.ancestors[(size_t)(first + i) * x.n_words + i / 32] >> (i % 32) & 1u);

@@ -1,5 +1,5 @@
 // Attention over trees of drafted tokens on the fifth-generation tensor cores (bfloat16, heads of 64 or 128 elements, pages of a multiple
-// of 64 keys, up to 128 query heads per kv head, up to 2,048 requests).
+// of 64 keys, up to 128 query heads per kv head).
 //
 // The rows of a row tile are the (node, query head of one kv group) pairs of consecutive nodes of one request, 128 of them at most, and
 // all see nearly the same keys: the request's settled tokens.  What has to be read is the cache, once a kv head, and that bounds the kernel up
@@ -14,7 +14,7 @@
 // Nothing stops between items: the rings and all barriers go on counting, and the loaders fetch the next item's keys while this one's end.
 //
 // Roles (12 warps):
-//   0        one lane loads K and V tiles into two rings            3        one lane loads the items' rows of q
+//   0        one lane loads K and V tiles into a ring               3        one lane loads the items' rows of q
 //   1, 2     one lane each issues S = Q K^T and O += P V of its half, scores two tiles ahead; P is read from tensor memory
 //   4 - 11   four softmax warps a half, one thread a row: scores by tcgen05.ld, scale, mask, running maximum (which moves only
 //            when it grows by more than 2^8) and sum in float32, P as bfloat16 over the scores it came from
@@ -41,12 +41,12 @@ constexpr int TMEM_COLS = 512;
 constexpr int GROUP_COLS = 256;         // tensor-memory columns of a half: S0, S1 (64 each), O
 constexpr float RESCALE_STEP = 8.f;     // log2 units
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MAX_SEGMENTS = 2048;
+constexpr int MAX_SEGMENTS = 640;       // requests of one launch (the line lies in shared memory); more take several
 
 // The line: what a key tile of a pair and of a single costs, what an item costs besides, the shortest part.
 constexpr int COST_PAIR = 3, COST_SINGLE = 2, COST_ITEM = 6;
 constexpr int PIECE = 3;                // key tiles: a cut closer to an item's end moves there
-constexpr int SHARE = 24;               // the shortest stretch, while there are blocks for every item
+constexpr int SHARE = 14;               // the shortest stretch, while there are blocks for every item
 
 __device__ int g_attn_tree_error = 0;
 }  // namespace
@@ -55,15 +55,22 @@ namespace {
 
 struct TreeCut {
     float* partial;                     // [blocks][2: a block's first part, its last][2 row tiles x (HD + 2) x 128]
-    int4* items;                        // [blocks][2]: where block i's first cut is the first within an item: (segment's first node of the item, nodes,
-};                                      // kv head, parts), (pair, -, -, -); no parts: none
+    int4* items;                        // [blocks]: where block i's beginning is the first cut within an item: (the item's first token, tokens, kv head,
+};                                      // parts); no parts: none
+
+// A block's part of the line, and the item that it begins in.
+struct Stretch {
+    unsigned line_end, sharers, each, rest, begin, end, at;
+    int seg, kvh, idx;
+    __device__ __forceinline__ unsigned cut(unsigned i) const { return i >= sharers ? line_end : each * i + rest * i / sharers; }     // line_end * i / sharers
+};
 __host__ __device__ constexpr size_t slot_floats(int head_dim) { return 2 * (size_t)(head_dim + 2) * BM; }
 
-__host__ __device__ constexpr int stages(int nkb) { return nkb == 1 ? 8 : 4; }
-template <bool B> struct Flag { static constexpr bool value = B; };
+constexpr int MAX_STAGES = 18;
+__host__ __device__ constexpr int stages(int nkb) { return nkb == 1 ? MAX_STAGES : MAX_STAGES / 2; }      // 144 KB of keys and values
 struct HalfBarriers { unsigned long long s_full[2], p_ready, pv_done, exp_done; };
 struct Barriers {
-    unsigned long long q_full, q_empty, k_full[8], k_empty[8], v_full[8], v_empty[8], state_ready, state_read;
+    unsigned long long q_full, q_empty, full[MAX_STAGES], empty[MAX_STAGES], state_ready, state_read;
     HalfBarriers g[2];
     unsigned tmem_base;
     int abort_flag;
@@ -71,6 +78,16 @@ struct Barriers {
 
 // An item, or the part of it that a block works on: key tiles [from, to) of `tiles`.
 struct Item { int seg, first, n, len, kvh, node0, nodes, k_begin, tiles, from, to; bool pair; };
+
+// The order in which an item's tiles go through the ring, which is the order in which they are used: a half issues the scores of its first two
+// tiles and then, tile by tile, the product with the values and the scores of the tile after next.  So the keys are `ahead` by 2 tiles
+// (4 where the halves share the tiles out), and then values and keys alternate.
+struct Order {
+    int n, ahead;
+    __device__ __forceinline__ Order(const Item& it) : n(it.to - it.from), ahead(min(n, it.pair ? 2 : 4)) {}
+    __device__ __forceinline__ int keys(int t) const { return t < ahead ? t : 2 * t - ahead + 1; }
+    __device__ __forceinline__ int values(int t) const { return ahead + t + min(t, n - ahead); }
+};
 
 __device__ __forceinline__ float row_scale_of(const AttentionParams& p, int tok, int head, float m, float l) {
     float shrink = 1.f;
@@ -82,33 +99,29 @@ __device__ __forceinline__ float row_scale_of(const AttentionParams& p, int tok,
     return shrink * gate_of(p, tok, head) / fmaxf(l, 1e-30f);
 }
 
-__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *(const unsigned*)&v;
-}
-
-// Element e of 64 bits in two words.
+// The n lowest of 64 bits.
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // NKB = head_dim / 64.  One block a multiprocessor.
-template <int NKB, bool CAP>
+template <int NKB, int FORM>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const AttentionParams p, const StepTokens b, const PagedCache c, const TreeStep x, const int tpt, const int q_box_tokens, const TreeCut cut,
                     const WaitControl waits) {
     constexpr int HD = 64 * NKB, ST = stages(NKB);
+    constexpr bool CAP = FORM != FORM_PLAIN, BIAS = FORM == FORM_ANY;      // (with a bias, a cap is chosen at run time)
     constexpr int Q_BYTES = NKB * BM * 128, KT_BYTES = NKB * BN * 128;
-    extern __shared__ __align__(1024) unsigned char smem[];     // [Q0][Q1][K ring][V ring], 1024-byte aligned, then the line
+    extern __shared__ __align__(1024) unsigned char smem[];     // [Q0][Q1][ring], 1024-byte aligned, then the line
     __shared__ Barriers bars;
     __shared__ float2 state_s[2][BM];                            // a single's two softmax states
-    __shared__ long long n_sets_s;
+    __shared__ Stretch stretch;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nq = p.num_heads, nkv = c.num_kv_heads, G = nq / nkv, S = x.n_segments;
     unsigned char* q_s = smem;
-    unsigned char* k_s = q_s + 2 * Q_BYTES;
-    unsigned char* v_s = k_s + ST * KT_BYTES;
-    long long* line = (long long*)(v_s + ST * KT_BYTES);         // [S + 1] what the requests before cost (for one kv head)
+    unsigned char* ring = q_s + 2 * Q_BYTES;
+    int4* const known = (int4*)(ring + ST * KT_BYTES);           // [S] a request's first node, nodes, settled tokens, key tiles
+    unsigned* line = (unsigned*)(known + S);                     // [S + 1] what the requests before cost (for one kv head)
     volatile int* abort_flag = &bars.abort_flag;
     int* const err = waits.error_word ? waits.error_word : &g_attn_tree_error;
     const long long limit = waits.limit_cycles;
@@ -118,8 +131,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         mbar_init(smem_u32(&bars.q_full), 1);
         mbar_init(smem_u32(&bars.q_empty), 2);
         for (int s = 0; s < ST; ++s) {
-            mbar_init(smem_u32(&bars.k_full[s]), 1); mbar_init(smem_u32(&bars.k_empty[s]), 2);      // both halves release a stage
-            mbar_init(smem_u32(&bars.v_full[s]), 1); mbar_init(smem_u32(&bars.v_empty[s]), 2);
+            mbar_init(smem_u32(&bars.full[s]), 1); mbar_init(smem_u32(&bars.empty[s]), 2);      // both halves release a stage
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(smem_u32(&bars.g[g].s_full[0]), 1); mbar_init(smem_u32(&bars.g[g].s_full[1]), 1);
@@ -132,157 +144,177 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         mbar_init_fence();
     }
     if (warp == 1) tmem_alloc(&bars.tmem_base, TMEM_COLS);
+    if (threadIdx.x == 3 * 32) {                                 // the tensor maps are needed first thing
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"((unsigned long long)&map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"((unsigned long long)&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"((unsigned long long)&map_v) : "memory");
+    }
     pdl_wait();
     pdl_launch_dependents();
 
     // ---- the line
-    struct Request { int first, n, len, k_begin, tiles, pairs, single; };
+    struct Request { int first, n, len, tiles, pairs, single; unsigned pair_len, single_len; };
     auto request_of = [&](int s) {
-        Request r;
-        r.first = min(max(x.cu_seqlens[s], 0), b.n_tokens);
-        r.n = min(max(x.cu_seqlens[s + 1], r.first), b.n_tokens) - r.first;
-        r.len = r.n ? max(b.positions[r.first], 0) : 0;
-        const int places = (int)min((long long)r.len + r.n, (long long)b.table_width * c.page_size);
-        r.k_begin = window_lowest(p.window_kind, p.window_size, r.len) / BN * BN;
-        r.tiles = r.n && places > r.k_begin ? (places - r.k_begin + BN - 1) / BN : 0;
-        const int row_tiles = r.tiles ? (r.n + tpt - 1) / tpt : 0;
-        r.pairs = row_tiles / 2;
-        r.single = row_tiles & 1;
-        return r;
+        const int4 v = known[s];
+        const int row_tiles = v.w ? (v.y + tpt - 1) / tpt : 0;
+        return Request{v.x, v.y, v.z, v.w, row_tiles / 2, row_tiles & 1, (unsigned)(COST_ITEM + v.w * COST_PAIR), (unsigned)(COST_ITEM + v.w * COST_SINGLE)};
     };
+    auto begin_of = [&](int len) { return window_lowest(p.window_kind, p.window_size, len) / BN * BN; };      // of the first key tile
     for (int s = threadIdx.x; s < S; s += THREADS) {
+        const int first = min(max(x.cu_seqlens[s], 0), b.n_tokens), n = min(max(x.cu_seqlens[s + 1], first), b.n_tokens) - first;
+        const int len = n ? max(b.positions[first], 0) : 0, k_begin = begin_of(len);
+        const int places = (int)min((long long)len + n, (long long)b.table_width * c.page_size);
+        known[s] = make_int4(first, n, len, n && places > k_begin ? (places - k_begin + BN - 1) / BN : 0);
         const Request r = request_of(s);
-        line[s + 1] = (long long)r.pairs * (COST_ITEM + (long long)r.tiles * COST_PAIR) + r.single * (COST_ITEM + (long long)r.tiles * COST_SINGLE);
+        line[s + 1] = r.pairs * r.pair_len + (r.single ? r.single_len : 0);
     }
     fence_before();
     __syncthreads();
     fence_after();
     const unsigned tmem = bars.tmem_base;
+    // the key tile where a cut `off` behind an item's beginning falls
+    auto tile_at = [](unsigned off, bool pair, int tiles) {
+        const int o = off <= COST_ITEM ? 0 : (int)off - COST_ITEM, t = pair ? (o + COST_PAIR / 2) / COST_PAIR : (o + COST_SINGLE / 2) / COST_SINGLE;
+        return t < PIECE ? 0 : tiles - t < PIECE ? tiles : t;
+    };
     if (warp == 0) {
-        long long sum = 0, sets = 0;
+        unsigned sum = 0, sets = 0;
         for (int s0 = 0; s0 < S; s0 += 32) {
-            long long v = s0 + lane < S ? line[s0 + lane + 1] : 0;
+            const bool there = s0 + lane < S;
+            unsigned v = there ? line[s0 + lane + 1] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, v, o);
+                const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
                 if (lane >= o) v += u;
             }
-            if (s0 + lane < S) {
+            if (there) {
                 line[s0 + lane + 1] = sum + v;
                 const Request r = request_of(s0 + lane);
                 sets += r.pairs + r.single;
             }
             sum += __shfl_sync(0xffffffffu, v, 31);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sets += __shfl_xor_sync(0xffffffffu, sets, o);
-        if (lane == 0) { line[0] = 0; n_sets_s = sets; }
+        sets = __reduce_add_sync(0xffffffffu, sets);
+        if (lane == 0) line[0] = 0;
+        __syncwarp();
+        if (lane == 0) {
+            // this block's stretch: of as many as there are items, or as shares of the shortest length; and the item that it begins in
+            Stretch t;
+            t.line_end = sum * nkv;
+            t.sharers = min(gridDim.x, max(sets * nkv, t.line_end / SHARE));
+            t.each = t.sharers ? t.line_end / t.sharers : 0;
+            t.rest = t.line_end - t.each * t.sharers;
+            t.begin = t.end = t.at = 0;
+            t.seg = t.kvh = t.idx = 0;
+            if (blockIdx.x < t.sharers && t.line_end) {
+                t.begin = t.cut(blockIdx.x);
+                t.end = t.cut(blockIdx.x + 1);
+                int lo = 0, hi = S;                              // nkv * line[lo] <= begin < nkv * line[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (nkv * line[mid] <= t.begin) lo = mid; else hi = mid;
+                }
+                const Request r = request_of(lo);
+                const unsigned per_head = line[lo + 1] - line[lo];
+                unsigned rest = t.begin - nkv * line[lo];
+                t.seg = lo;
+                t.kvh = rest / per_head;
+                rest -= t.kvh * per_head;
+                t.idx = min((unsigned)r.pairs, rest / r.pair_len);
+                t.at = t.begin - (rest - t.idx * r.pair_len);
+            }
+            stretch = t;
+        }
     }
     __syncthreads();
-    const long long line_end = line[S] * nkv;
-    // as many blocks as there are items, or as shares of the shortest length
-    const int sharers = (int)min((long long)gridDim.x, max(n_sets_s * nkv, line_end / SHARE));
-    struct Place { Item item; long long at; int len; };          // the item's beginning on the line and its length
-    auto place_of = [&](long long t) {                           // 0 <= t < line_end
-        int lo = 0, hi = S;                                      // nkv * line[lo] <= t < nkv * line[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (nkv * line[mid] <= t) lo = mid; else hi = mid;
-        }
-        const Request r = request_of(lo);
-        const long long per_head = line[lo + 1] - line[lo];
-        long long rest = t - nkv * line[lo];
-        Place q;
-        q.item.kvh = (int)(rest / per_head);
-        q.at = nkv * line[lo] + q.item.kvh * per_head;
-        rest -= q.item.kvh * per_head;
-        const int pair_len = COST_ITEM + r.tiles * COST_PAIR, idx = (int)min((long long)r.pairs, rest / pair_len);
-        q.item.pair = idx < r.pairs;
-        q.at += (long long)idx * pair_len;
-        q.len = q.item.pair ? pair_len : COST_ITEM + r.tiles * COST_SINGLE;
-        q.item.seg = lo; q.item.first = r.first; q.item.n = r.n; q.item.len = r.len; q.item.k_begin = r.k_begin; q.item.tiles = r.tiles;
-        q.item.node0 = 2 * idx * tpt;
-        q.item.nodes = min((q.item.pair ? 2 : 1) * tpt, r.n - q.item.node0);
-        q.item.from = 0; q.item.to = r.tiles;
-        return q;
-    };
-    // the key tile where a cut `off` behind an item's beginning falls
-    auto tile_at = [&](long long off, const Item& it) {
-        const int w = it.pair ? COST_PAIR : COST_SINGLE;
-        const int t = off <= COST_ITEM ? 0 : (int)((off - COST_ITEM + w / 2) / w);
-        return t < PIECE ? 0 : it.tiles - t < PIECE ? it.tiles : t;
-    };
-    auto cut_at = [&](int i) { return i >= sharers ? line_end : line_end * i / sharers; };
-    const long long begin = (int)blockIdx.x < sharers && line_end > 0 ? cut_at(blockIdx.x) : 0;
-    const long long end = (int)blockIdx.x < sharers && line_end > 0 ? cut_at(blockIdx.x + 1) : 0;
-    if (threadIdx.x == 0) {
-        int4 a = make_int4(0, 0, 0, 0), d = make_int4(0, 0, 0, 0);
-        if (begin < end) {
-            const Place q = place_of(begin);
-            const int mine = tile_at(begin - q.at, q.item);
-            if (mine > 0 && mine < q.item.tiles) {               // the cuts within the item
-                int first = -1, n = 0;
-                for (int i = (int)(q.at * sharers / line_end); i < sharers; ++i) {
-                    const long long t = cut_at(i);
-                    if (t >= q.at + q.len) break;
-                    if (t <= q.at) continue;
-                    const int at = tile_at(t - q.at, q.item);
-                    if (at == 0 || at == q.item.tiles) continue;
-                    if (n++ == 0) first = i;
-                }
-                if (first == (int)blockIdx.x) {
-                    a = make_int4(q.item.first + q.item.node0, q.item.nodes, q.item.kvh, n + 1);
-                    d.x = q.item.pair;
+    // every role goes over the block's items alike; f returns false to give up
+    auto for_items = [&](auto f) {
+        const unsigned begin = stretch.begin, end = stretch.end;
+        if (begin >= end) return;
+        int seg = stretch.seg, kvh = stretch.kvh, idx = stretch.idx;
+        unsigned at = stretch.at;
+        Request r = request_of(seg);
+        while (true) {
+            Item it;
+            it.pair = idx < r.pairs;
+            const unsigned len = it.pair ? r.pair_len : r.single_len;
+            it.seg = seg; it.kvh = kvh; it.first = r.first; it.n = r.n; it.len = r.len; it.k_begin = begin_of(r.len); it.tiles = r.tiles;
+            it.node0 = 2 * idx * tpt;
+            it.nodes = min((it.pair ? 2 : 1) * tpt, r.n - it.node0);
+            it.from = at < begin ? tile_at(begin - at, it.pair, r.tiles) : 0;
+            it.to = at + len > end ? tile_at(end - at, it.pair, r.tiles) : r.tiles;
+            if (it.from < it.to && !f(it)) return;
+            at += len;
+            if (at >= end) return;
+            if (++idx == r.pairs + r.single) {                   // the next kv head, the next request that has anything
+                idx = 0;
+                if (++kvh == nkv) {
+                    kvh = 0;
+                    do ++seg; while (line[seg + 1] == line[seg]);
+                    r = request_of(seg);
                 }
             }
         }
-        cut.items[2 * blockIdx.x] = a;
-        cut.items[2 * blockIdx.x + 1] = d;
-    }
-    // every role goes over the block's items alike; f returns false to give up
-    auto for_items = [&](auto f) {
-        for (long long t = begin; t < end;) {
-            Place q = place_of(t);
-            if (t == begin) q.item.from = tile_at(t - q.at, q.item);
-            if (q.at + q.len > end) q.item.to = tile_at(end - q.at, q.item);
-            t = q.at + q.len;
-            if (q.item.from < q.item.to && !f(q.item)) return;
-        }
     };
+    if (warp == 11) {
+        // for the second kernel, ahead of this warp's rows: is this block's beginning the first cut within an item?
+        int4 a = make_int4(0, 0, 0, 0);
+        if (stretch.begin < stretch.end) {
+            const Request r = request_of(stretch.seg);
+            const bool pair = stretch.idx < r.pairs;
+            const unsigned at = stretch.at, len = pair ? r.pair_len : r.single_len;
+            auto within = [&](unsigned i) {
+                const unsigned t = stretch.cut(i);
+                if (t <= at || t >= at + len) return false;
+                const int tile = tile_at(t - at, pair, r.tiles);
+                return tile > 0 && tile < r.tiles;
+            };
+            if (within(blockIdx.x)) {
+                int cuts = 0, before = 0;
+                for (unsigned i = lane; i < stretch.sharers; i += 32)
+                    if (within(i)) { ++cuts; before += i < blockIdx.x; }
+                cuts = __reduce_add_sync(0xffffffffu, cuts);
+                before = __reduce_add_sync(0xffffffffu, before);
+                const int node0 = 2 * stretch.idx * tpt;
+                if (before == 0) a = make_int4(r.first + node0, min((pair ? 2 : 1) * tpt, r.n - node0), stretch.kvh, cuts + 1);
+            }
+        }
+        if (lane == 0) cut.items[blockIdx.x] = a;
+    }
     auto wait = [&](unsigned long long& bar, unsigned parity, int code) { return mbar_wait(smem_u32(&bar), parity & 1, abort_flag, err, code, limit); };
 
     if (warp == 0) {
         if (lane == 0) {
             // ---- keys and values
-            unsigned kc = 0;                                     // tiles of the block so far
-            unsigned issued_k = 0, issued_v = 0;
+            unsigned at = 0;                                     // tiles put into the ring so far
             for_items([&](const Item& it) {
+                const Order order(it);
                 const int* table = b.block_table + (size_t)it.seg * b.table_width;
-                for (int i = it.from; i < it.to; ++i, ++kc) {
-                    const int j0 = it.k_begin + i * BN, s = kc % ST;
+                auto load = [&](const CUtensorMap* map, int t) {
+                    const int j0 = it.k_begin + (it.from + t) * BN, s = at % ST;
                     int page = table[j0 / c.page_size];
                     if (page < 0 || page >= c.n_pages) page = 0;           // (no page: nothing there is visible to a row)
                     const int y = (page * nkv + it.kvh) * c.page_size + j0 % c.page_size;
-                    if (!wait(bars.k_empty[s], kc / ST + 1, 1)) return false;
-                    mbar_expect_tx(smem_u32(&bars.k_full[s]), KT_BYTES);
+                    if (!wait(bars.empty[s], at / ST + 1, 1)) return false;
+                    mbar_expect_tx(smem_u32(&bars.full[s]), KT_BYTES);
 #pragma unroll
-                    for (int kb = 0; kb < NKB; ++kb) tma_load_2d(smem_u32(k_s + s * KT_BYTES + kb * BN * 128), &map_k, kb * 64, y, smem_u32(&bars.k_full[s]));
-                    ++issued_k;
-                    if (!wait(bars.v_empty[s], kc / ST + 1, 1)) return false;
-                    mbar_expect_tx(smem_u32(&bars.v_full[s]), KT_BYTES);
-#pragma unroll
-                    for (int kb = 0; kb < NKB; ++kb) tma_load_2d(smem_u32(v_s + s * KT_BYTES + kb * BN * 128), &map_v, kb * 64, y, smem_u32(&bars.v_full[s]));
-                    ++issued_v;
+                    for (int kb = 0; kb < NKB; ++kb) tma_load_2d(smem_u32(ring + s * KT_BYTES + kb * BN * 128), map, kb * 64, y, smem_u32(&bars.full[s]));
+                    ++at;
+                    return true;
+                };
+                for (int t = 0; t < order.ahead; ++t)
+                    if (!load(&map_k, t)) return false;
+                for (int t = 0; t < order.n; ++t) {
+                    if (!load(&map_v, t)) return false;
+                    if (t + order.ahead < order.n && !load(&map_k, t + order.ahead)) return false;
                 }
                 return true;
             });
             // the last releases must have arrived, or (where the block gives up) the copies in flight have landed, before it leaves
-            for (unsigned j = kc > ST ? kc - ST : 0; j < kc && !*abort_flag; ++j)
-                if (!wait(bars.k_empty[j % ST], j / ST, 1) || !wait(bars.v_empty[j % ST], j / ST, 1)) break;
-            if (*abort_flag) {
-                for (unsigned j = issued_k > ST ? issued_k - ST : 0; j < issued_k; ++j) mbar_drain(smem_u32(&bars.k_full[j % ST]), (j / ST) & 1, limit);
-                for (unsigned j = issued_v > ST ? issued_v - ST : 0; j < issued_v; ++j) mbar_drain(smem_u32(&bars.v_full[j % ST]), (j / ST) & 1, limit);
-            }
+            for (unsigned j = at > ST ? at - ST : 0; j < at && !*abort_flag; ++j)
+                if (!wait(bars.empty[j % ST], j / ST, 1)) break;
+            if (*abort_flag)
+                for (unsigned j = at > ST ? at - ST : 0; j < at; ++j) mbar_drain(smem_u32(&bars.full[j % ST]), (j / ST) & 1, limit);
         }
     } else if (warp == 3) {
         if (lane == 0) {
@@ -309,36 +341,37 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             HalfBarriers& gb = bars.g[g];
             const unsigned tmem_g = tmem + g * GROUP_COLS;
             const unsigned idesc_s = make_idesc(BM, BN), idesc_pv = make_idesc(BM, HD, true);
-            unsigned n_items = 0, kp = 0, vp = 0;                // items; key and value tiles of the block released so far
+            unsigned n_items = 0, at = 0;                        // items; tiles of the ring released so far
             unsigned scored = 0, added = 0;                      // own tiles whose scores, whose products with the values are issued
             for_items([&](const Item& it) {
-                const int n = it.to - it.from, step = it.pair ? 1 : 2, first = it.pair ? 0 : g, own = n > first ? (n - first + step - 1) / step : 0;
-                const unsigned base = kp;
+                const Order order(it);
+                const int n = order.n, step = it.pair ? 1 : 2, first = it.pair ? 0 : g, own = n > first ? (n - first + step - 1) / step : 0;
+                const unsigned base = at;
                 unsigned char* q_g = q_s + (it.pair ? g : 0) * Q_BYTES;
-                // a tile of the other half's: wait until it has landed (so that the halves drift apart by no more than the ring) and hand it back
-                auto pass = [&](unsigned long long* full, unsigned long long* empty, unsigned& at, unsigned to) {
+                // tiles of the other half's: wait until they have landed (so that the halves drift apart by no more than the ring) and hand them back
+                auto pass_to = [&](unsigned to) {
                     for (; at < to; ++at) {
-                        if (!wait(full[at % ST], at / ST, 2)) return false;
-                        mbar_arrive(smem_u32(&empty[at % ST]));
+                        if (!wait(bars.full[at % ST], at / ST, 2)) return false;
+                        mbar_arrive(smem_u32(&bars.empty[at % ST]));
                     }
                     return true;
                 };
                 auto issue_scores = [&](int li) {
-                    if (!pass(bars.k_full, bars.k_empty, kp, base + first + li * step)) return false;
-                    const int s = kp % ST, sb = scored & 1;
-                    if (!wait(bars.k_full[s], kp / ST, 2)) return false;
+                    if (!pass_to(base + order.keys(first + li * step))) return false;
+                    const int s = at % ST, sb = scored & 1;
                     // P of two tiles before lay where the scores go; the product issued last is waited for (by parity only that can be)
                     if (added > 0 && !wait(gb.pv_done, added - 1, 2)) return false;
+                    if (!wait(bars.full[s], at / ST, 2)) return false;
                     fence_after();
-                    const unsigned qa = smem_u32(q_g), ka = smem_u32(k_s + s * KT_BYTES);
+                    const unsigned qa = smem_u32(q_g), ka = smem_u32(ring + s * KT_BYTES);
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks)
                         mma(tmem_g + sb * BN, smem_desc_k_major(qa + (ks / 4) * BM * 128 + (ks % 4) * 32),
                             smem_desc_k_major(ka + (ks / 4) * BN * 128 + (ks % 4) * 32), idesc_s, ks > 0 ? 1u : 0u);
                     commit(smem_u32(&gb.s_full[sb]));
-                    commit(smem_u32(&bars.k_empty[s]));
+                    commit(smem_u32(&bars.empty[s]));
                     if (li == own - 1) commit(smem_u32(&bars.q_empty));
-                    ++kp;
+                    ++at;
                     ++scored;
                     return true;
                 };
@@ -347,23 +380,23 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (own > 0 && !issue_scores(0)) return false;
                 if (own > 1 && !issue_scores(1)) return false;
                 for (int li = 0; li < own; ++li) {
-                    if (!pass(bars.v_full, bars.v_empty, vp, base + first + li * step)) return false;
-                    const int s = vp % ST;
-                    if (!wait(gb.p_ready, added, 2) || !wait(bars.v_full[s], vp / ST, 2)) return false;
+                    if (!pass_to(base + order.values(first + li * step))) return false;
+                    const int s = at % ST;
+                    if (!wait(gb.p_ready, added, 2) || !wait(bars.full[s], at / ST, 2)) return false;
                     fence_after();
-                    const unsigned va = smem_u32(v_s + s * KT_BYTES);
+                    const unsigned va = smem_u32(ring + s * KT_BYTES);
 #pragma unroll
                     for (int ks = 0; ks < BN / 16; ++ks)
                         mma_a_tmem(tmem_g + 2 * BN, tmem_g + (added & 1) * BN + ks * 8, smem_desc(va + ks * 16 * 128, BN * 128, 1024), idesc_pv,
                                    (li > 0 || ks > 0) ? 1u : 0u);
                     commit(smem_u32(&gb.pv_done));
-                    commit(smem_u32(&bars.v_empty[s]));
-                    ++vp;
+                    commit(smem_u32(&bars.empty[s]));
+                    ++at;
                     ++added;
                     if (li + 2 < own && !issue_scores(li + 2)) return false;
                 }
                 ++n_items;
-                return pass(bars.k_full, bars.k_empty, kp, base + n) && pass(bars.v_full, bars.v_empty, vp, base + n);
+                return pass_to(base + 2 * n);
             });
         }
     } else {
@@ -373,13 +406,14 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const unsigned lane_base = tmem + g * GROUP_COLS + ((unsigned)(quarter * 32) << 16);
         const float scale = p.softmax_scale * LOG2E;
         // cap and slope in units of the raw scores (see the prompts' kernel)
-        const float cap_raw = CAP ? p.score_softcap / p.softmax_scale : 0.f, inv_cap_raw = CAP ? p.softmax_scale / p.score_softcap : 0.f;
-        const float cap_arg = CAP ? 2.f * LOG2E * p.softmax_scale / p.score_softcap : 0.f;
-        const bool biased = p.head_slopes != nullptr;
-        unsigned tile0 = 0, seen = 0, singles = 0, turns = 0;    // tiles of the block before this item; own tiles so far; singles, a pair's tiles so far
+        const bool capped = CAP && p.score_softcap > 0.f, biased = BIAS && p.head_slopes != nullptr;
+        const float cap_raw = capped ? p.score_softcap / p.softmax_scale : 0.f, inv_cap_raw = capped ? p.softmax_scale / p.score_softcap : 0.f;
+        const float cap_arg = capped ? 2.f * LOG2E * p.softmax_scale / p.score_softcap : 0.f;
+        unsigned ring0 = 0, seen = 0, singles = 0, turns = 0;    // tiles of the ring before this item; own tiles so far; singles, a pair's tiles so far
         auto all_wait = [&](unsigned long long& bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, wait(bar, parity, 3)); };
         for_items([&](const Item& it) {
-            const int n = it.to - it.from, step = it.pair ? 1 : 2, first = it.pair ? 0 : g, own = n > first ? (n - first + step - 1) / step : 0;
+            const Order order(it);
+            const int n = order.n, step = it.pair ? 1 : 2, first = it.pair ? 0 : g, own = n > first ? (n - first + step - 1) / step : 0;
             const bool part = it.from > 0 || it.to < it.tiles;
             const int node_base = it.node0 + (it.pair ? g * tpt : 0), nodes = max(0, min(tpt, it.node0 + it.nodes - node_base));
             const int n_rows = nodes * G;
@@ -400,9 +434,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     live = (unsigned long long)__ballot_sync(0xffffffffu, holds(b0 + lane)) |
                            (unsigned long long)__ballot_sync(0xffffffffu, holds(b0 + 32 + lane)) << 32;
                     if (live != ~0ull) {
-                        const unsigned kt = tile0 + i;
-                        if (!all_wait(bars.v_full[kt % ST], kt / ST)) return false;
-                        unsigned char* v_t = v_s + (kt % ST) * KT_BYTES;
+                        const unsigned at = ring0 + order.values(i);
+                        if (!all_wait(bars.full[at % ST], at / ST)) return false;
+                        unsigned char* v_t = ring + (at % ST) * KT_BYTES;
                         for (int e = r; e < BN * 8 * NKB; e += BM) {
                             const int row = e / (8 * NKB), ch = e % (8 * NKB);
                             if (!(live >> row & 1)) *(uint4*)(v_t + (ch / 8) * BN * 128 + row * 128 + (ch % 8) * 16) = make_uint4(0, 0, 0, 0);
@@ -423,7 +457,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 float s[BN];
                 ld64(s, lane_base + sb * BN);
                 const bool open = j0 >= lo_all && j0 + BN <= it.len;      // every key visible to every row
-                if (CAP) {
+                if (capped) {
                     // cap tanh(s scale / cap): the series where every score of the warp's rows is small against the cap, else by 2^x
                     float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -494,28 +528,19 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 unsigned packed[BN / 2];
                 f2 sum2[4] = {0ull, 0ull, 0ull, 0ull};
                 const f2 scale2 = pack2(scale, scale), neg_m2 = pack2(neg_m, neg_m);
-                auto weights = [&](auto mixed) {
 #pragma unroll
-                    for (int e = 0; e < BN; e += 2) {
-                        if (e == BN * 3 / 4) {
-                            __syncwarp();
-                            if (it.pair && lane == 0) mbar_arrive(smem_u32(&gb.exp_done));
-                        }
-                        const f2 y = fma2(pack2(s[e], s[e + 1]), scale2, neg_m2);
-                        float a, bb;
-                        // three of sixteen pairs on the multiply-add units (not where a masked key must get 0)
-                        if (decltype(mixed)::value && ((e / 2) % 16 == 3 || (e / 2) % 16 == 8 || (e / 2) % 16 == 13)) {
-                            ex2_pair(y, a, bb);
-                        } else {
-                            unpack2(y, a, bb);
-                            a = ex2(a);
-                            bb = ex2(bb);
-                        }
-                        sum2[(e >> 1) & 3] = add2(sum2[(e >> 1) & 3], pack2(a, bb));
-                        packed[e / 2] = pack_bf16(a, bb);
+                for (int e = 0; e < BN; e += 2) {
+                    if (e == BN * 3 / 4) {
+                        __syncwarp();
+                        if (it.pair && lane == 0) mbar_arrive(smem_u32(&gb.exp_done));
                     }
-                };
-                if (open) weights(Flag<true>{}); else weights(Flag<false>{});
+                    float a, d;
+                    unpack2(fma2(pack2(s[e], s[e + 1]), scale2, neg_m2), a, d);
+                    a = ex2(a);
+                    d = ex2(d);
+                    sum2[(e >> 1) & 3] = add2(sum2[(e >> 1) & 3], pack2(a, d));
+                    packed[e / 2] = pack_bf16(a, d);
+                }
                 float sum_a, sum_b;
                 unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_a, sum_b);
                 l += sum_a + sum_b;
@@ -601,7 +626,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (!all_wait(bars.state_read, singles)) return false;       // before either output is written again
                 ++singles;
             }
-            tile0 += n;
+            ring0 += 2 * n;
             return true;
         });
     }
@@ -613,38 +638,38 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
-// Adds up the parts of the items that were cut, in the order of the keys.  grid (blocks, head_dim / JOIN_COLS), a thread a row; part 0 of an item
-// is the last of the block before its first cut, part k the first of the block behind its cut k.
-constexpr int JOIN_COLS = 16;
-__global__ void __launch_bounds__(2 * BM) attn_tree_tc_join_kernel(const AttentionParams p, const TreeCut cut, int nkv, int tpt, int hd) {
+// Adds up the parts of the items that were cut, in the order of the keys.  grid (blocks, head_dim / JOIN_COLS, row tiles of a pair), a thread a row;
+// part 0 of an item is the last of the block before its first cut, part k the first of the block behind its cut k.  What it costs is the latency of
+// its loads, so as many as there are registers for are asked for at once.
+constexpr int JOIN_COLS = 8;
+__global__ void __launch_bounds__(BM) attn_tree_tc_join_kernel(const AttentionParams p, const TreeCut cut, int nkv, int tpt, int hd) {
     pdl_wait();
     pdl_launch_dependents();
-    const int4 item = __ldcg(cut.items + 2 * blockIdx.x);
+    const int4 item = __ldcg(cut.items + blockIdx.x);
     if (item.w < 2) return;
-    const int G = p.num_heads / nkv, g = threadIdx.x / BM, r = threadIdx.x % BM, c0 = blockIdx.y * JOIN_COLS;
-    if (r >= min(tpt, item.y - g * tpt) * G) return;
+    const int G = p.num_heads / nkv, g = blockIdx.z, r = threadIdx.x, c0 = blockIdx.y * JOIN_COLS;
+    if (r >= min(tpt, item.y - g * tpt) * G) return;             // (a single's second row tile has no rows)
     const int tok = item.x + g * tpt + r / G, head = item.z * G + r % G;
-    auto slot = [&](int k) { return cut.partial + (2 * (size_t)blockIdx.x + 2 * k - (k ? 2 : 1)) * slot_floats(hd); };
+    const float* parts = cut.partial + (size_t)(2 * blockIdx.x) * slot_floats(hd);
+    auto slot = [&](int k) { return parts + (k ? 2 * (long long)k - 2 : -1ll) * (long long)slot_floats(hd); };
     float m = -INFINITY, l = 0.f, o[JOIN_COLS];
 #pragma unroll
     for (int e = 0; e < JOIN_COLS; ++e) o[e] = 0.f;
-    constexpr int N = 4;                                         // parts whose loads are asked for together
+    constexpr int N = 12;                                        // parts whose loads are asked for together
     for (int k0 = 0; k0 < item.w; k0 += N) {
         float2 ml[N];
         float v[N][JOIN_COLS];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const float* from = slot(min(k0 + k, item.w - 1));
-            ml[k] = __ldcg((const float2*)(from + 2 * hd * BM) + threadIdx.x);
+            if (k0 + k >= item.w) { ml[k] = make_float2(-INFINITY, 0.f); continue; }
+            const float* from = slot(k0 + k);
+            ml[k] = __ldcg((const float2*)(from + 2 * hd * BM) + g * BM + r);
 #pragma unroll
             for (int e = 0; e < JOIN_COLS; ++e) v[k][e] = __ldcg(from + (size_t)(g * hd + c0 + e) * BM + r);
         }
         float top = m;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            if (k0 + k >= item.w) ml[k].x = -INFINITY;
-            top = fmaxf(top, ml[k].x);
-        }
+        for (int k = 0; k < N; ++k) top = fmaxf(top, ml[k].x);
         const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
         m = top;
         l *= keep;
@@ -652,7 +677,7 @@ __global__ void __launch_bounds__(2 * BM) attn_tree_tc_join_kernel(const Attenti
         for (int e = 0; e < JOIN_COLS; ++e) o[e] *= keep;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if (ml[k].x == -INFINITY) continue;                  // (a part without a key of this row)
+            if (ml[k].x == -INFINITY) continue;                  // (no part, or one without a key of this row)
             const float w = exp2f(ml[k].x - m);
             l = fmaf(w, ml[k].y, l);
 #pragma unroll
@@ -660,11 +685,8 @@ __global__ void __launch_bounds__(2 * BM) attn_tree_tc_join_kernel(const Attenti
         }
     }
     const float inv = row_scale_of(p, tok, head, m, l);
-    __nv_bfloat16* dst = (__nv_bfloat16*)p.out + out_row_of(p, tok, head) * hd + c0;
-#pragma unroll
-    for (int e = 0; e < JOIN_COLS; e += 8)
-        *(uint4*)(dst + e) = make_uint4(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv),
-                                        pack_bf16(o[e + 4] * inv, o[e + 5] * inv), pack_bf16(o[e + 6] * inv, o[e + 7] * inv));
+    *(uint4*)((__nv_bfloat16*)p.out + out_row_of(p, tok, head) * hd + c0) =
+        make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv), pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
 }
 
 template <int NKB>
@@ -685,32 +707,41 @@ int launch(const AttentionParams& p, const StepTokens& b, const PagedCache& c, c
         if (!make_map(&mk, c.kv, 2, dims, strides, box)) return SPITE_LAUNCH_FAILED;
         if (!make_map(&mv, (const __nv_bfloat16*)c.kv + c.v_offset, 2, dims, strides, box)) return SPITE_LAUNCH_FAILED;
     }
-    const size_t smem = (2 * (size_t)NKB * BM + 2 * stages(NKB) * (size_t)NKB * BN) * 128 + (size_t)(x.n_segments + 1) * 8;
-    auto k = p.score_softcap > 0.f ? attn_tree_tc_kernel<NKB, true> : attn_tree_tc_kernel<NKB, false>;
+    const size_t smem = (2 * (size_t)NKB * BM + stages(NKB) * (size_t)NKB * BN) * 128 + (size_t)(x.n_segments < MAX_SEGMENTS ? x.n_segments : MAX_SEGMENTS) * 20 + 4;
+    auto k = p.head_slopes ? attn_tree_tc_kernel<NKB, FORM_ANY> : p.score_softcap > 0.f ? attn_tree_tc_kernel<NKB, FORM_CAP> : attn_tree_tc_kernel<NKB, FORM_PLAIN>;
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SPITE_LAUNCH_FAILED;
-    SPITE_LAUNCH(k, n_sm, THREADS, smem, st, mq, mk, mv, p, b, c, x, tpt, box_tokens, cut, s_waits);
-    SPITE_LAUNCH(attn_tree_tc_join_kernel, dim3(n_sm, hd / JOIN_COLS), 2 * BM, 0, st, p, cut, nkv, tpt, hd);
+    const long long tiles = (long long)b.table_width * c.page_size / BN;
+    for (int s0 = 0; s0 < x.n_segments; s0 += MAX_SEGMENTS) {
+        TreeStep some = x;
+        StepTokens tokens = b;
+        some.cu_seqlens += s0;
+        some.n_segments = x.n_segments - s0 < MAX_SEGMENTS ? x.n_segments - s0 : MAX_SEGMENTS;
+        tokens.block_table += (size_t)s0 * b.table_width;
+        SPITE_LAUNCH(k, n_sm, THREADS, smem, st, mq, mk, mv, p, tokens, c, some, tpt, box_tokens, cut, s_waits);
+        if (tiles >= 2 * PIECE)                                  // (with fewer no item is cut)
+            SPITE_LAUNCH(attn_tree_tc_join_kernel, dim3(n_sm, hd / JOIN_COLS, 2), BM, 0, st, p, cut, nkv, tpt, hd);
+    }
     return spite_launch_status();
 }
 
 }  // namespace
 
-// `n_sm`: number of multiprocessors (a block each).  `scratch`: n_sm * (4 * (head_dim + 2) * 128 + 8) floats.
-SPITE_API int spite_tree_attention_tc(const AttentionParams* p, const StepTokens* b, const PagedCache* c, const TreeStep* x, int n_sm, float* scratch,
-                                      long long n_floats, void* stream) {
-    if (!p || !b || !c || !x || !p->q || !p->out || !c->kv || !b->positions || !b->block_table || !x->cu_seqlens || !x->ancestors || !scratch || n_sm < 1)
-        return SPITE_BAD_ARG;
-    if (b->n_tokens < 0 || b->table_width < 1 || c->n_pages < 1 || c->page_size < 1 || x->n_segments < 1 || x->n_words < 1) return SPITE_BAD_ARG;
-    if (p->num_heads < 1 || c->num_kv_heads < 1 || p->num_heads % c->num_kv_heads) return SPITE_BAD_ARG;
-    if (p->window_kind < 0 || p->window_kind > 2 || (p->window_kind != SPITE_WINDOW_FULL && p->window_size < 1)) return SPITE_BAD_ARG;
-    const int G = p->num_heads / c->num_kv_heads;
-    if ((c->head_dim != 64 && c->head_dim != 128) || G > BM || c->page_size % BN || x->n_segments > MAX_SEGMENTS) return SPITE_UNSUPPORTED;
-    if (p->distance_bias || c->key_scale || c->v_offset == 0) return SPITE_UNSUPPORTED;
-    if ((long long)c->n_pages * c->num_kv_heads * c->page_size > 0x7fffffffll) return SPITE_UNSUPPORTED;       // TMA coordinates are int32
-    if ((((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)c->kv | (uintptr_t)scratch) & 15) || (c->v_offset & 7)) return SPITE_UNSUPPORTED;
-    const long long slots = 2ll * n_sm * (long long)slot_floats(c->head_dim);
-    if (slots + 8ll * n_sm > n_floats) return SPITE_BAD_ARG;
-    if (b->n_tokens == 0) return SPITE_OK;
+// `n_sm`: number of multiprocessors (a block each).  `scratch`: n_sm * (4 * (head_dim + 2) * 128 + 4) floats.
+SPITE_API int spite_tree_attention_tc(const TreeCall* call, int n_sm, float* scratch, long long n_floats, void* stream) {
+    if (!call || !scratch || n_sm < 1 || !tree_call_ok(*call)) return SPITE_BAD_ARG;
+    const AttentionParams& p = call->p;
+    const PagedCache& c = call->c;
+    if ((c.head_dim != 64 && c.head_dim != 128) || p.num_heads / c.num_kv_heads > BM || c.page_size % BN) return SPITE_UNSUPPORTED;
+    if (p.distance_bias || c.key_scale || c.v_offset == 0) return SPITE_UNSUPPORTED;
+    if ((long long)c.n_pages * c.num_kv_heads * c.page_size > 0x7fffffffll) return SPITE_UNSUPPORTED;       // TMA coordinates are int32
+    if ((((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)c.kv | (uintptr_t)scratch) & 15) || (c.v_offset & 7)) return SPITE_UNSUPPORTED;
+    const long long slots = 2ll * n_sm * (long long)slot_floats(c.head_dim);
+    if (slots + 4ll * n_sm > n_floats) return SPITE_BAD_ARG;
+    // the line is counted in 32 bits: no request has more key tiles than its table, no more row tiles than nodes
+    const long long tiles = (long long)call->b.table_width * c.page_size / BN + 1;
+    const double longest = (double)(COST_ITEM + COST_PAIR * tiles) * c.num_kv_heads * (call->b.n_tokens / (BM / (p.num_heads / c.num_kv_heads)) + call->x.n_segments);
+    if (longest >= 4e9) return SPITE_UNSUPPORTED;
+    if (call->b.n_tokens == 0) return SPITE_OK;
     const TreeCut cut{scratch, (int4*)(scratch + slots)};
-    return c->head_dim == 64 ? launch<1>(*p, *b, *c, *x, cut, n_sm, (cudaStream_t)stream) : launch<2>(*p, *b, *c, *x, cut, n_sm, (cudaStream_t)stream);
+    return c.head_dim == 64 ? launch<1>(p, call->b, c, call->x, cut, n_sm, (cudaStream_t)stream) : launch<2>(p, call->b, c, call->x, cut, n_sm, (cudaStream_t)stream);
 }

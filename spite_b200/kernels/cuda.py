@@ -10,6 +10,7 @@ import ctypes as C
 import functools
 import math
 import os
+import struct
 
 import torch
 
@@ -144,33 +145,12 @@ class AttnDecodeExtra(C.Structure):
                 ("seg_min_tokens", C.c_int), ("seg_max_tokens", C.c_int), ("cache_settled", C.c_int)]
 
 
-class TreeStep(C.Structure):
-    _fields_ = [("cu_seqlens", C.c_void_p), ("ancestors", C.c_void_p), ("n_segments", C.c_int), ("n_words", C.c_int)]
-
-
-class LayoutParams(C.Structure):
-    _fields_ = [("tables", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p), ("n_free", C.c_void_p),
-                ("slots", C.c_void_p), ("lengths", C.c_void_p), ("new_tokens", C.c_void_p), ("parents", C.c_void_p),
-                ("block_table", C.c_void_p), ("cu_seqlens", C.c_void_p), ("positions", C.c_void_p), ("seg_of_token", C.c_void_p),
-                ("slot_map", C.c_void_p), ("ancestors", C.c_void_p), ("status", C.c_void_p),
-                ("n_rows", C.c_int), ("table_width", C.c_int), ("n_pages", C.c_int), ("n_requests", C.c_int), ("out_width", C.c_int),
-                ("n_tokens", C.c_int), ("n_parents", C.c_int), ("n_words", C.c_int), ("page_size", C.c_int), ("window_kind", C.c_int),
-                ("window_size", C.c_int)]
-
-
-class AcceptGroup(C.Structure):
-    _fields_ = [("kv", C.c_void_p), ("key_scales", C.c_void_p), ("slot_map", C.c_void_p), ("plane_bytes", C.c_longlong),
-                ("planes", C.c_int), ("caches", C.c_int), ("n_pages", C.c_int), ("num_kv_heads", C.c_int), ("page_size", C.c_int),
-                ("row_bytes", C.c_int)]
-
-
-class AcceptParams(C.Structure):
-    MAX_GROUPS = 8
-    _fields_ = [("tokens", C.c_void_p), ("parents", C.c_void_p), ("targets", C.c_void_p), ("cu_seqlens", C.c_void_p),
-                ("counts", C.c_void_p), ("path", C.c_void_p), ("emitted", C.c_void_p), ("slots", C.c_void_p),
-                ("lengths", C.c_void_p), ("lengths_out", C.c_void_p),
-                ("n_tokens", C.c_int), ("n_requests", C.c_int), ("depth", C.c_int), ("n_rows", C.c_int), ("n_groups", C.c_int),
-                ("groups", AcceptGroup * MAX_GROUPS)]
+# The arguments of the calls of a step of drafted tokens, packed as the C structures lie in memory.
+_TREE_CALL = struct.Struct("PPiiififPPPifPPi4x" "PPPii" "PqiiiiP" "PPii")         # AttentionParams, StepTokens, PagedCache, TreeStep
+_LAYOUT_CALL = struct.Struct("15P11i4x")                                          # LayoutParams
+_ACCEPT_GROUPS = 8
+_ACCEPT_GROUP = struct.Struct("PPPq6i")                                           # AcceptGroup
+_ACCEPT_CALL = struct.Struct(f"10P5i4x{_ACCEPT_GROUPS * _ACCEPT_GROUP.size}s")    # AcceptParams
 
 
 class SampleParams(C.Structure):
@@ -199,6 +179,10 @@ def _error_buffer():
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _check(status, what):
@@ -348,6 +332,7 @@ class CudaKernels(KernelSet):
         self.device = torch.device(device)
         self._dt = _DT[dtype]
         self._libs = {}
+        self._entries = {}
         self.launches = 0          # kernels launched so far (for measurement reports)
         self.attention_scratch_bytes = 0   # partial results of the last split-key attention call
         self.launches_by_library = collections.Counter()   # the same, by kernel library
@@ -1098,8 +1083,7 @@ class CudaKernels(KernelSet):
         self._count("attention", 1)
         _check(st, "turn_heads")
 
-    def _attention_params(self, what, q, out, num_heads, window, softmax_scale, sink_logit, head_sinks, head_slopes, head_gates, out_by_head,
-                          score_softcap, distance_bias):
+    def _check_attention(self, what, q, out, num_heads, softmax_scale, head_sinks, head_slopes, head_gates, score_softcap, distance_bias):
         self._t(q, self.dtype, "q"); self._t(out, self.dtype, "out")
         if score_softcap is not None and not score_softcap > 0:
             raise KernelError(f"{what}: the cap of the scores must be positive")
@@ -1116,6 +1100,11 @@ class CudaKernels(KernelSet):
             if tuple(self._t(distance_bias.padded, torch.float32, "distance_bias.padded").shape) != \
                     (num_heads, distance_bias.length + 2 * distance_bias.PAD):
                 raise KernelError(f"{what}: one row of numbers by distance per head")
+
+    def paged_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, cache_settled=False,
+                        sink_logit=None, head_sinks=None, head_slopes=None, head_gates=None, out_by_head=False,
+                        score_softcap=None, distance_bias=None):
+        self._check_attention("paged_attention", q, out, num_heads, softmax_scale, head_sinks, head_slopes, head_gates, score_softcap, distance_bias)
         p = AttentionParams(q=q.data_ptr(), out=out.data_ptr(), num_heads=num_heads,
                             window_kind=_WINDOW[window.kind], window_size=int(window.size),
                             softmax_scale=float(softmax_scale),
@@ -1126,13 +1115,6 @@ class CudaKernels(KernelSet):
         if distance_bias is not None:
             p.distance_bias, p.distance_runs = distance_bias.padded.data_ptr(), distance_bias.runs.data_ptr()
             p.distance_len = distance_bias.length
-        return p
-
-    def paged_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, cache_settled=False,
-                        sink_logit=None, head_sinks=None, head_slopes=None, head_gates=None, out_by_head=False,
-                        score_softcap=None, distance_bias=None):
-        p = self._attention_params("paged_attention", q, out, num_heads, window, softmax_scale, sink_logit, head_sinks, head_slopes, head_gates,
-                                   out_by_head, score_softcap, distance_bias)
         b, c = self._step_tokens(batch, cache.group), self._paged(cache)
         group = num_heads // c.num_kv_heads
         if (self.dtype == torch.bfloat16 and c.head_dim % 16 == 0 and c.head_dim <= 128 and group <= 16
@@ -1261,139 +1243,165 @@ class CudaKernels(KernelSet):
         self._count("attention_decode", 1)
         _check(st, "paged_attention (decode)")
 
+    # The calls of a step of drafted tokens stand between its other launches, where the host's time counts as much as the kernels': their
+    # arguments are packed in one go (0.3 us; a ctypes structure by field names 1.7) and go through entries with declared types.
+    def _entry(self, library, name, *argtypes):
+        f = self._entries.get(name)
+        if f is None:
+            f = self._entries[name] = getattr(self._lib(library), name)
+            f.argtypes = argtypes
+        return f
+
+    def _whole_numbers(self, what, tensors, dtype=torch.int32):
+        """`tensors`: (name, tensor, dimensions), contiguous tensors of `dtype` on the device."""
+        for name, t, dims in tensors:
+            if not (t.is_cuda and t.is_contiguous() and t.dtype is dtype and t.dim() == dims):
+                raise KernelError(f"{what}: {name} must be a contiguous CUDA tensor of {dtype} with {dims} dimensions")
+
+    def _on_current_device(self, what, t) -> int:
+        """The current stream's handle; the launch goes to the current device, which has to be the tensors'."""
+        if t.get_device() != torch.cuda.current_device():
+            raise KernelError(f"{what}: the tensors are on {t.device}, the current device is another")
+        return self._raw_stream()
+
     def tree_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, sink_logit=None, head_sinks=None, head_slopes=None,
                        head_gates=None, out_by_head=False, score_softcap=None, distance_bias=None):
-        p = self._attention_params("tree_attention", q, out, num_heads, window, softmax_scale, sink_logit, head_sinks, head_slopes, head_gates,
-                                   out_by_head, score_softcap, distance_bias)
-        M, table = batch.n_tokens, batch.block_tables[cache.group]
-        S = batch.cu_seqlens.numel() - 1
-        if batch.ancestors is None:
-            raise KernelError("tree_attention: the step has no ancestor sets")
-        for name, t, size in (("positions", batch.positions, M), ("seg_of_token", batch.seg_of_token, M), ("cu_seqlens", batch.cu_seqlens, 2),
-                              ("block_table", table, S), ("ancestors", batch.ancestors, M)):
-            if self._t(t, torch.int32, name).numel() < size:
-                raise KernelError(f"tree_attention: {name} has {t.numel()} elements for {M} tokens of {S} requests")
-        if table.dim() != 2 or table.shape[0] < S or batch.ancestors.dim() != 2 or batch.ancestors.shape[0] < M or not batch.ancestors.shape[1]:
-            raise KernelError("tree_attention: block_table is [requests, pages], ancestors [tokens, words]")
-        b, c = self._step_tokens(batch, cache.group), self._paged(cache)
-        if q.shape[0] != M or q.numel() != M * num_heads * c.head_dim or num_heads % c.num_kv_heads:
-            raise KernelError(f"tree_attention: q {tuple(q.shape)} does not hold {M} tokens of {num_heads} heads of {c.head_dim} ({c.num_kv_heads} kv heads)")
-        if c.head_dim > 256:
-            raise KernelError(f"tree_attention: heads of {c.head_dim} elements; up to 256 are supported")
+        what = "tree_attention"
+        self._check_attention(what, q, out, num_heads, softmax_scale, head_sinks, head_slopes, head_gates, score_softcap, distance_bias)
+        M, table, cu, positions, seg, sets = batch.n_tokens, batch.block_tables[cache.group], batch.cu_seqlens, batch.positions, batch.seg_of_token, batch.ancestors
+        if sets is None:
+            raise KernelError(f"{what}: the step has no ancestor sets")
+        self._whole_numbers(what, (("positions", positions, 1), ("seg_of_token", seg, 1), ("cu_seqlens", cu, 1), ("block_table", table, 2), ("ancestors", sets, 2)))
+        kv, scales = cache.kv, cache.key_scale
+        self._t(kv, self.dtype, "cache")
+        planes, n_pages, kv_heads, page, hd = kv.shape
+        S, (rows, width), (n_sets, n_words) = cu.numel() - 1, table.shape, sets.shape
+        if S < 1 or rows < S or not width or positions.numel() < M or seg.numel() < M or n_sets < M or not n_words:
+            raise KernelError(f"{what}: positions, seg_of_token and ancestors of {M} tokens and block_table of {S} requests are needed")
+        if scales is not None and tuple(self._t(scales, torch.float32, "key_scale").shape) != (n_pages, kv_heads, page):
+            raise KernelError("a cache's key factors are [pages, kv heads, page_size]")
+        if q.shape[0] != M or q.numel() != M * num_heads * hd or num_heads % kv_heads:
+            raise KernelError(f"{what}: q {tuple(q.shape)} does not hold {M} tokens of {num_heads} heads of {hd} ({kv_heads} kv heads)")
+        if hd > 256:
+            raise KernelError(f"{what}: heads of {hd} elements; up to 256 are supported")
         if not M:
             return
-        x = TreeStep(cu_seqlens=batch.cu_seqlens.data_ptr(), ancestors=batch.ancestors.data_ptr(), n_segments=S, n_words=batch.ancestors.shape[1])
-        if (self.dtype == torch.bfloat16 and c.head_dim in (64, 128) and c.page_size % 64 == 0 and self.use_tcgen05_attention
-                and distance_bias is None and cache.kv.shape[0] == 2 and cache.key_scale is None):
-            n_floats = self.sm_count * (4 * (c.head_dim + 2) * 128 + 8)
+        stream = self._on_current_device(what, q)
+        has_sink = sink_logit is not None or head_sinks is not None
+        call = _TREE_CALL.pack(
+            q.data_ptr(), out.data_ptr(), num_heads, _WINDOW[window.kind], window.size, softmax_scale, has_sink, sink_logit or 0.0,
+            _address(head_sinks), _address(head_slopes), _address(head_gates), M if out_by_head else 0, score_softcap or 0.0,
+            0 if distance_bias is None else distance_bias.padded.data_ptr(), 0 if distance_bias is None else distance_bias.runs.data_ptr(),
+            0 if distance_bias is None else distance_bias.length,
+            positions.data_ptr(), seg.data_ptr(), table.data_ptr(), width, M,
+            kv.data_ptr(), kv.stride(0) if planes == 2 else 0, n_pages, page, kv_heads, hd, _address(scales),
+            cu.data_ptr(), sets.data_ptr(), S, n_words)
+        if self.dtype is torch.bfloat16 and (hd == 64 or hd == 128) and page % 64 == 0 and planes == 2 and scales is None and distance_bias is None \
+                and self.use_tcgen05_attention:
+            n_floats = self.sm_count * (4 * (hd + 2) * 128 + 4)
             part = torch.empty(n_floats, dtype=torch.float32, device=q.device)
-            st = self._lib("attention_tree_tc").spite_tree_attention_tc(C.byref(p), C.byref(b), C.byref(c), C.byref(x), self.sm_count, C.c_void_p(part.data_ptr()),
-                                                                        C.c_longlong(n_floats), self._stream())
-            if st != -2:                        # -2: more than 128 heads a kv head, 2,048 requests, a row that does not start at 16 bytes
+            st = self._entry("attention_tree_tc", "spite_tree_attention_tc", C.c_char_p, C.c_int, C.c_void_p, C.c_longlong, C.c_void_p)(
+                call, self.sm_count, part.data_ptr(), n_floats, stream)
+            if st != -2:                        # -2: more than 128 heads a kv head, a tensor that does not start at 16 bytes, sizes beyond 32 bits
                 self._count("attention_tree_tc", 2)
-                _check(st, "tree_attention (tcgen05)")
+                _check(st, f"{what} (tcgen05)")
                 return
         # The multiply-add kernel: shares of the keys so that about eight blocks a multiprocessor run, none shorter than four tiles
         # of 32 keys if the table is full.
-        group = num_heads // c.num_kv_heads
-        blocks = max(1, -(-M * min(group, 16) // 16)) * -(-group // 16) * c.num_kv_heads
-        keys = min(table.shape[1] * c.page_size, batch.context_bucket or (1 << 30))
+        group = num_heads // kv_heads
+        blocks = max(1, -(-M * min(group, 16) // 16)) * -(-group // 16) * kv_heads
+        keys = min(width * page, batch.context_bucket or (1 << 30))
         if window.kind != "full":
-            keys = min(keys, window.size + 32 * x.n_words)
+            keys = min(keys, window.size + 32 * n_words)
         splits = max(1, min(32, 8 * self.sm_count // blocks, keys // 128))
-        part = torch.empty(M * num_heads * splits * (c.head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-        st = self._lib("attention_tree").spite_tree_attention(self._dt, C.byref(p), C.byref(b), C.byref(c), C.byref(x), C.c_void_p(_ptr(part)),
-                                                              C.c_longlong(0 if part is None else part.numel()), splits, self._stream())
+        part = torch.empty(M * num_heads * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        st = self._entry("attention_tree", "spite_tree_attention", C.c_int, C.c_char_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p)(
+            self._dt, call, _address(part), 0 if part is None else part.numel(), splits, stream)
         self._count("attention_tree", 1 + (splits > 1))
-        _check(st, "tree_attention")
+        _check(st, what)
 
     # ------------------------------------------------------------------ steps laid out and drafts accepted on the device
-    def _ints(self, what, dtype=torch.int32, **tensors):
-        """The tensors named, checked to be contiguous whole numbers on the device with the number of dimensions given: name=(tensor, dimensions)."""
-        for name, (t, dims) in tensors.items():
-            if self._t(t, dtype, f"{what}: {name}").dim() != dims:
-                raise KernelError(f"{what}: {name} has {t.dim()} dimensions, {dims} are needed")
-
     def layout_step(self, pages, slots, lengths, new_tokens, out, *, parents=None):
-        what = "layout_step"
-        self._ints(what, tables=(pages.tables, 2), held=(pages.held, 1), slots=(slots, 1), lengths=(lengths, 1), new_tokens=(new_tokens, 1),
-                   block_table=(out.block_table, 2), cu_seqlens=(out.cu_seqlens, 1), positions=(out.positions, 1),
-                   seg_of_token=(out.seg_of_token, 1), status=(out.status, 1))
-        self._ints(what, torch.int64, slot_map=(out.slot_map, 1))
-        if (pages.free_pages is None) != (pages.n_free is None):
+        what, tables, held, free, n_free = "layout_step", pages.tables, pages.held, pages.free_pages, pages.n_free
+        block, cu, positions, seg, sets, status = out.block_table, out.cu_seqlens, out.positions, out.seg_of_token, out.ancestors, out.status
+        self._whole_numbers(what, (("tables", tables, 2), ("held", held, 1), ("slots", slots, 1), ("lengths", lengths, 1), ("new_tokens", new_tokens, 1),
+                                   ("block_table", block, 2), ("cu_seqlens", cu, 1), ("positions", positions, 1), ("seg_of_token", seg, 1), ("status", status, 1)))
+        self._whole_numbers(what, (("slot_map", out.slot_map, 1),), torch.int64)
+        if (free is None) != (n_free is None):
             raise KernelError(f"{what}: a stack of free pages needs its height, and the other way round")
-        if pages.free_pages is not None:
-            self._ints(what, free_pages=(pages.free_pages, 1), n_free=(pages.n_free, 1))
+        if free is not None:
+            self._whole_numbers(what, (("free_pages", free, 1), ("n_free", n_free, 1)))
         if parents is not None:
-            self._ints(what, parents=(parents, 1))
-        if out.ancestors is not None:
-            self._ints(what, ancestors=(out.ancestors, 2))
-        S, (R, W), M = slots.numel(), pages.tables.shape, out.positions.numel()
-        if pages.held.numel() != R or lengths.numel() != R or new_tokens.numel() != S or out.block_table.shape[0] != S or out.cu_seqlens.numel() != S + 1:
+            self._whole_numbers(what, (("parents", parents, 1),))
+        if sets is not None:
+            self._whole_numbers(what, (("ancestors", sets, 2),))
+        S, (R, W), M, (block_rows, out_width) = slots.numel(), tables.shape, positions.numel(), block.shape
+        n_sets, n_words = (M, 0) if sets is None else sets.shape
+        if held.numel() != R or lengths.numel() != R or new_tokens.numel() != S or block_rows != S or cu.numel() != S + 1:
             raise KernelError(f"{what}: {S} requests in {R} rows: held and lengths have a number a row, new_tokens and block_table one a request, cu_seqlens one more")
-        if out.seg_of_token.numel() != M or out.slot_map.numel() != M or (out.ancestors is not None and out.ancestors.shape[0] != M):
+        if seg.numel() != M or out.slot_map.numel() != M or n_sets != M:
             raise KernelError(f"{what}: positions, seg_of_token, slot_map and ancestors have room for the same number of tokens")
-        if out.status.numel() != 1 or (pages.n_free is not None and pages.n_free.numel() != 1):
+        if status.numel() != 1 or (n_free is not None and n_free.numel() != 1):
             raise KernelError(f"{what}: status and n_free are one number each")
-        if int(pages.page_size) < 1 or not W or not out.block_table.shape[1] or (out.ancestors is not None and not out.ancestors.shape[1]):
-            raise KernelError(f"{what}: empty pages, tables or sets")
-        if not S:
-            raise KernelError(f"{what}: a step needs a request")
+        if not S or not W or not out_width or pages.page_size < 1 or (sets is not None and not n_words):
+            raise KernelError(f"{what}: a step needs requests, and pages, tables and sets that are not empty")
+        stream = self._on_current_device(what, slots)
         plan = torch.empty(S, dtype=torch.int32, device=slots.device)
-        p = LayoutParams(tables=pages.tables.data_ptr(), held=pages.held.data_ptr(), free_pages=_ptr(pages.free_pages), n_free=_ptr(pages.n_free),
-                         slots=slots.data_ptr(), lengths=lengths.data_ptr(), new_tokens=new_tokens.data_ptr(), parents=_ptr(parents),
-                         block_table=out.block_table.data_ptr(), cu_seqlens=out.cu_seqlens.data_ptr(), positions=out.positions.data_ptr(),
-                         seg_of_token=out.seg_of_token.data_ptr(), slot_map=out.slot_map.data_ptr(), ancestors=_ptr(out.ancestors),
-                         status=out.status.data_ptr(), n_rows=R, table_width=W, n_pages=0 if pages.free_pages is None else pages.free_pages.numel(),
-                         n_requests=S, out_width=out.block_table.shape[1], n_tokens=M, n_parents=0 if parents is None else parents.numel(),
-                         n_words=0 if out.ancestors is None else out.ancestors.shape[1], page_size=int(pages.page_size),
-                         window_kind=_WINDOW[pages.window.kind], window_size=int(pages.window.size))
-        st = self._lib("drafts").spite_layout_step(C.byref(p), C.c_void_p(plan.data_ptr()), self._stream())
+        call = _LAYOUT_CALL.pack(
+            tables.data_ptr(), held.data_ptr(), _address(free), _address(n_free), slots.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), _address(parents),
+            block.data_ptr(), cu.data_ptr(), positions.data_ptr(), seg.data_ptr(), out.slot_map.data_ptr(), _address(sets), status.data_ptr(),
+            R, W, 0 if free is None else free.numel(), S, out_width, M, 0 if parents is None else parents.numel(), n_words, pages.page_size,
+            _WINDOW[pages.window.kind], pages.window.size)
+        st = self._entry("drafts", "spite_layout_step", C.c_char_p, C.c_void_p, C.c_void_p)(call, plan.data_ptr(), stream)
         self._count("drafts", 2)
         _check(st, what)
 
     def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
         what = "accept_drafts"
-        self._ints(what, tokens=(tokens, 1), targets=(targets, 1), cu_seqlens=(cu_seqlens, 1), counts=(counts, 1), path=(path, 2), emitted=(emitted, 2))
-        S, M = cu_seqlens.numel() - 1, tokens.numel()
+        self._whole_numbers(what, (("tokens", tokens, 1), ("targets", targets, 1), ("cu_seqlens", cu_seqlens, 1), ("counts", counts, 1), ("path", path, 2),
+                                   ("emitted", emitted, 2)))
+        S, M, (rows, depth) = cu_seqlens.numel() - 1, tokens.numel(), path.shape
         if parents is not None:
-            self._ints(what, parents=(parents, 1))
+            self._whole_numbers(what, (("parents", parents, 1),))
         if targets.numel() != M or (parents is not None and parents.numel() != M):
             raise KernelError(f"{what}: {M} tokens have a parent and a target each")
-        if S < 1 or counts.numel() != S or path.shape != emitted.shape or path.shape[0] != S or not path.shape[1]:
+        if S < 1 or counts.numel() != S or rows != S or not depth or emitted.shape != path.shape:
             raise KernelError(f"{what}: {S} requests: counts has a number, path and emitted a row of the same length for each")
         if (lengths is None) != (lengths_out is None):
             raise KernelError(f"{what}: lengths and lengths_out go together")
         if slots is not None:
-            self._ints(what, slots=(slots, 1))
+            self._whole_numbers(what, (("slots", slots, 1),))
             if slots.numel() != S:
                 raise KernelError(f"{what}: {slots.numel()} slots for {S} requests")
+        n_rows = 0
         if lengths is not None:
-            self._ints(what, lengths=(lengths, 1), lengths_out=(lengths_out, 1))
-            if lengths.numel() != lengths_out.numel() or (slots is None and lengths.numel() < S):
+            self._whole_numbers(what, (("lengths", lengths, 1), ("lengths_out", lengths_out, 1)))
+            n_rows = lengths.numel()
+            if n_rows != lengths_out.numel() or (slots is None and n_rows < S):
                 raise KernelError(f"{what}: lengths and lengths_out have a number a row")
-        if len(caches) > AcceptParams.MAX_GROUPS:
-            raise KernelError(f"{what}: {len(caches)} groups of caches; up to {AcceptParams.MAX_GROUPS} in one call")
-        p = AcceptParams(tokens=tokens.data_ptr(), parents=_ptr(parents), targets=targets.data_ptr(), cu_seqlens=cu_seqlens.data_ptr(),
-                         counts=counts.data_ptr(), path=path.data_ptr(), emitted=emitted.data_ptr(), slots=_ptr(slots), lengths=_ptr(lengths),
-                         lengths_out=_ptr(lengths_out), n_tokens=M, n_requests=S, depth=path.shape[1],
-                         n_rows=0 if lengths is None else lengths.numel(), n_groups=len(caches))
-        most = 1
-        for g, (kv, slot_map, scales) in enumerate(caches):
+        if len(caches) > _ACCEPT_GROUPS:
+            raise KernelError(f"{what}: {len(caches)} groups of caches; up to {_ACCEPT_GROUPS} in one call")
+        groups, most = [], 1
+        for kv, slot_map, scales in caches:
             if self._t(kv, self.dtype, f"{what}: cache").dim() != 6 or not kv.numel():
                 raise KernelError(f"{what}: a cache is [caches, planes, pages, kv heads, page_size, head_dim]")
-            self._ints(what, torch.int64, slot_map=(slot_map, 1))
+            self._whole_numbers(what, (("slot_map", slot_map, 1),), torch.int64)
             if slot_map.numel() < M:
                 raise KernelError(f"{what}: the slot map has {slot_map.numel()} rows for {M} tokens")
-            n, planes, n_pages, heads, page_size, size = kv.shape
-            if scales is not None and tuple(self._t(scales, torch.float32, f"{what}: key_scales").shape) != (n, n_pages, heads, page_size):
+            n, planes, n_pages, heads, page, size = kv.shape
+            if scales is not None and tuple(self._t(scales, torch.float32, f"{what}: key_scales").shape) != (n, n_pages, heads, page):
                 raise KernelError(f"{what}: key_scales are [caches, pages, kv heads, page_size]")
-            p.groups[g] = AcceptGroup(kv=kv.data_ptr(), key_scales=_ptr(scales), slot_map=slot_map.data_ptr(), plane_bytes=kv.stride(1) * kv.element_size(),
-                                      planes=n * planes, caches=n, n_pages=n_pages, num_kv_heads=heads, page_size=page_size, row_bytes=size * kv.element_size())
-            most = max(most, n * planes * heads * size * kv.element_size() // 16)
+            row_bytes = size * kv.element_size()
+            groups.append(_ACCEPT_GROUP.pack(kv.data_ptr(), _address(scales), slot_map.data_ptr(), n_pages * heads * page * row_bytes, n * planes, n, n_pages,
+                                             heads, page, row_bytes))
+            most = max(most, n * planes * heads * row_bytes // 16)
+        stream = self._on_current_device(what, tokens)
+        call = _ACCEPT_CALL.pack(tokens.data_ptr(), _address(parents), targets.data_ptr(), cu_seqlens.data_ptr(), counts.data_ptr(), path.data_ptr(),
+                                 emitted.data_ptr(), _address(slots), _address(lengths), _address(lengths_out), M, S, depth, n_rows, len(groups),
+                                 b"".join(groups))
         # a thread for every 16 bytes of a token's rows, as long as that is not far more blocks than the device holds
         pieces = max(1, min(-(-most // 256), max(1, 16 * self.sm_count // S)))
-        st = self._lib("drafts").spite_accept_drafts(C.byref(p), pieces, self._stream())
+        st = self._entry("drafts", "spite_accept_drafts", C.c_char_p, C.c_int, C.c_void_p)(call, pieces, stream)
         self._count("drafts", 1)
         _check(st, what)
 

@@ -117,6 +117,11 @@ def test_largest_trees(kernels, dtype, size, nodes):
     run(kernels, TreeCase([100], [nodes], heads=2, kv_heads=1, size=size, dtype=dtype, seed=2))
 
 
+@pytest.mark.parametrize("dtype,size", [(BF, 64), (F32, 16)])
+def test_many_requests(kernels, dtype, size):
+    run(kernels, TreeCase([(37 * s) % 150 for s in range(1000)], [s % 4 for s in range(1000)], heads=2, kv_heads=1, size=size, dtype=dtype, seed=8))
+
+
 @pytest.mark.parametrize("dtype,heads,size", [(BF, 5, 128), (BF, 8, 64), (F32, 2, 64)])
 def test_long_contexts_are_shared_among_blocks(kernels, dtype, heads, size):
     """Contexts that are cut along the keys, beside ones that are not."""
