@@ -1306,15 +1306,15 @@ class CudaKernels(KernelSet):
                 self._count("attention_tree_tc", 2)
                 _check(st, f"{what} (tcgen05)")
                 return
-        # The multiply-add kernel: shares of the keys so that about eight blocks a multiprocessor run, none shorter than four tiles
-        # of 32 keys if the table is full.
+        # The float32 kernel: blocks of 32 rows and shares of the keys, as many as two blocks a multiprocessor take at once, none shorter than two
+        # tiles of 64 keys if the table is full.
         group = num_heads // kv_heads
-        blocks = max(1, -(-M * min(group, 16) // 16)) * -(-group // 16) * kv_heads
+        blocks = (M // max(1, 32 // group) + S) * -(-group // 32) * kv_heads
         keys = min(width * page, batch.context_bucket or (1 << 30))
         if window.kind != "full":
             keys = min(keys, window.size + 32 * n_words)
-        splits = max(1, min(32, 8 * self.sm_count // blocks, keys // 128))
-        part = torch.empty(M * num_heads * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        splits = max(1, min(32, 2 * self.sm_count // blocks, keys // 128))
+        part = torch.empty(M * num_heads * splits * (-(-hd // 4) * 4 + 4), dtype=torch.float32, device=q.device) if splits > 1 else None
         st = self._entry("attention_tree", "spite_tree_attention", C.c_int, C.c_char_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p)(
             self._dt, call, _address(part), 0 if part is None else part.numel(), splits, stream)
         self._count("attention_tree", 1 + (splits > 1))
