@@ -56,7 +56,7 @@ template <typename T, int BN> constexpr size_t smem_bytes(int hd8) {
 // partial [tokens, heads, shares, part_floats].
 template <typename T, int HD4, bool ASYNC>
 __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionParams p, const StepTokens b, const PagedCache c, const TreeStep x,
-                                                            float* partial, const int nodes_per_block, const int n_splits) {
+                                                            float* partial, const int nodes_per_block, const int n_splits, const int share_tiles) {
     constexpr int BN = 64 / HD4, KT = BN / 32;                // keys of a tile; eights of them of a warp
     constexpr bool REST = sizeof(T) == 4;                      // (bfloat16 has none)
     extern __shared__ __align__(16) unsigned char smem[];
@@ -110,7 +110,15 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
     const int places = (int)min((long long)len + node0 + nt, (long long)b.table_width * c.page_size);
     const int lo_any = window_lowest(p.window_kind, p.window_size, len);
     const int n_tiles = places > lo_any ? (places - lo_any + BN - 1) / BN : 0, split_no = blockIdx.z;
-    const int tile0 = (int)((long long)n_tiles * split_no / n_splits), tile1 = (int)((long long)n_tiles * (split_no + 1) / n_splits);
+    // (shares of so many tiles, the last one of the rest: a short request has fewer of them, and their blocks leave at once)
+    const int tile0 = min(n_tiles, split_no * share_tiles), tile1 = split_no == n_splits - 1 ? n_tiles : min(n_tiles, tile0 + share_tiles);
+    if (tile0 == tile1 && n_splits > 1) {                      // nothing in this share: its rows' maximum says so
+        for (int r = threadIdx.x; r < n_rows; r += THREADS)
+            __stcg((float2*)(partial + (((size_t)(t0 + r / heads) * nq + kvh * G + h0 + r % heads) * n_splits + split_no) * part_floats(hd) + hdp),
+                   make_float2(-INFINITY, 0.f));
+        return;
+    }
+
     // where a tile's keys lie: a thread a key, asked for a tile ahead and written down later
     struct Key { long long row; int at, node; float factor; };
     auto find = [&](int ti) {
@@ -377,12 +385,15 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_tree_join_kernel(const Atte
     for (int e = 0; e < HD4; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
     auto ask = [&](int s0) {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
+        for (int k = 0; k < N; ++k) {
+            const float share_m = __shfl_sync(0xffffffffu, ml.x, (s0 + k) & 31);
+            const bool there = s0 + k < n_splits && share_m > -INFINITY;       // (a share without a key of this row has left nothing)
 #pragma unroll
             for (int e = 0; e < HD4; ++e) {
                 const int d = 4 * (lane + 32 * e);
-                v[k][e] = s0 + k < n_splits && d < hdp ? __ldcg((const float4*)(part + (s0 + k) * part_floats(hd) + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[k][e] = there && d < hdp ? __ldcg((const float4*)(part + (s0 + k) * part_floats(hd) + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
+        }
     };
     ask(0);
     const float m = warp_max(ml.x);
@@ -416,7 +427,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_tree_join_kernel(const Atte
 }
 
 template <typename T, int HD4>
-int launch(const TreeCall& a, float* partial, int n_splits, cudaStream_t st) {
+int launch(const TreeCall& a, float* partial, int n_splits, int share_keys, cudaStream_t st) {
     const AttentionParams& p = a.p;
     const PagedCache& c = a.c;
     const int hd = c.head_dim, G = p.num_heads / c.num_kv_heads, chunks = (G + ROWS - 1) / ROWS;
@@ -427,7 +438,7 @@ int launch(const TreeCall& a, float* partial, int n_splits, cudaStream_t st) {
     const dim3 grid(a.b.n_tokens / nodes + a.x.n_segments, c.num_kv_heads * chunks, n_splits);       // (no request has a chunk more than fill it)
     auto k = async ? attn_tree_kernel<T, HD4, true> : attn_tree_kernel<T, HD4, false>;
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SPITE_LAUNCH_FAILED;
-    SPITE_LAUNCH(k, grid, THREADS, smem, st, p, a.b, c, a.x, partial, nodes, n_splits);
+    SPITE_LAUNCH(k, grid, THREADS, smem, st, p, a.b, c, a.x, partial, nodes, n_splits, (share_keys + 64 / HD4 - 1) / (64 / HD4));
     if (n_splits > 1)
         SPITE_LAUNCH((attn_tree_join_kernel<T, HD4>), dim3(a.b.n_tokens, (p.num_heads + 3) / 4), JOIN_THREADS, 0, st, p, a.x, (const float*)partial, hd, n_splits);
     return spite_launch_status();
@@ -435,18 +446,18 @@ int launch(const TreeCall& a, float* partial, int n_splits, cudaStream_t st) {
 
 }  // namespace
 
-// `partial` (16-byte aligned): tokens * heads * n_splits * (head_dim rounded up to four, + 4) floats where n_splits (1..32) > 1.
-SPITE_API int spite_tree_attention(int dtype, const TreeCall* call, float* partial, long long n_partial, int n_splits, void* stream) {
+// `n_splits` shares of `share_keys` keys, the last one of the rest.  `partial` (16-byte aligned): tokens * heads * n_splits * (head_dim rounded up to four, + 4) floats where n_splits (1..32) > 1.
+SPITE_API int spite_tree_attention(int dtype, const TreeCall* call, float* partial, long long n_partial, int n_splits, int share_keys, void* stream) {
     if (!call || !tree_call_ok(*call)) return SPITE_BAD_ARG;
     const AttentionParams& p = call->p;
     const int hd = call->c.head_dim;
-    if (n_splits < 1 || n_splits > 32) return SPITE_BAD_ARG;
+    if (n_splits < 1 || n_splits > 32 || share_keys < 1) return SPITE_BAD_ARG;
     if (n_splits > 1 && (!partial || ((uintptr_t)partial & 15) || n_partial < (long long)call->b.n_tokens * p.num_heads * n_splits * part_floats(hd)))
         return SPITE_BAD_ARG;
     if (hd > 256 || p.num_heads > 4 * 65535) return SPITE_UNSUPPORTED;
     if (call->b.n_tokens == 0) return SPITE_OK;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == SPITE_DT_F32) return hd <= 128 ? launch<float, 1>(*call, partial, n_splits, st) : launch<float, 2>(*call, partial, n_splits, st);
-    if (dtype == SPITE_DT_BF16) return hd <= 128 ? launch<__nv_bfloat16, 1>(*call, partial, n_splits, st) : launch<__nv_bfloat16, 2>(*call, partial, n_splits, st);
+    if (dtype == SPITE_DT_F32) return hd <= 128 ? launch<float, 1>(*call, partial, n_splits, share_keys, st) : launch<float, 2>(*call, partial, n_splits, share_keys, st);
+    if (dtype == SPITE_DT_BF16) return hd <= 128 ? launch<__nv_bfloat16, 1>(*call, partial, n_splits, share_keys, st) : launch<__nv_bfloat16, 2>(*call, partial, n_splits, share_keys, st);
     return SPITE_BAD_ARG;
 }

@@ -1306,17 +1306,18 @@ class CudaKernels(KernelSet):
                 self._count("attention_tree_tc", 2)
                 _check(st, f"{what} (tcgen05)")
                 return
-        # The float32 kernel: blocks of 32 rows and shares of the keys, as many as two blocks a multiprocessor take at once, none shorter than two
-        # tiles of 64 keys if the table is full.
+        # The float32 kernel: blocks of 32 rows and shares of the keys, of 128 or as many more as keep the blocks of full tables at eight a
+        # multiprocessor (two run at once; requests are shorter than their tables, and the blocks of shares they do not have leave at once).
         group = num_heads // kv_heads
         blocks = (M // max(1, 32 // group) + S) * -(-group // 32) * kv_heads
         keys = min(width * page, batch.context_bucket or (1 << 30))
         if window.kind != "full":
             keys = min(keys, window.size + 32 * n_words)
-        splits = max(1, min(32, 2 * self.sm_count // blocks, keys // 128))
+        splits = max(1, min(32, 8 * self.sm_count // blocks, -(-keys // 128)))
+        share = -(-keys // splits)
         part = torch.empty(M * num_heads * splits * (-(-hd // 4) * 4 + 4), dtype=torch.float32, device=q.device) if splits > 1 else None
-        st = self._entry("attention_tree", "spite_tree_attention", C.c_int, C.c_char_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p)(
-            self._dt, call, _address(part), 0 if part is None else part.numel(), splits, stream)
+        st = self._entry("attention_tree", "spite_tree_attention", C.c_int, C.c_char_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p)(
+            self._dt, call, _address(part), 0 if part is None else part.numel(), splits, share, stream)
         self._count("attention_tree", 1 + (splits > 1))
         _check(st, what)
 
