@@ -34,7 +34,8 @@ struct LayoutParams {
 
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32;
+constexpr int FEW_PAGES = 4;             // that a request's own thread takes
 
 __device__ __forceinline__ int first_needed(const LayoutParams& p, int len) {       // (a later token reads nothing before it)
     if (p.window_kind == 1) return len / p.window_size * p.window_size;
@@ -43,7 +44,7 @@ __device__ __forceinline__ int first_needed(const LayoutParams& p, int len) {   
 }
 
 // Sums over the block's threads before this one, of three counts; the totals are added to `total`.
-__device__ __forceinline__ void scan3(int (&v)[3], int (*scratch)[3], long long (&total)[3], long long (&before)[3]) {
+__device__ void scan3(const int (&v)[3], int (*scratch)[3], long long (&total)[3], long long (&before)[3]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl[3];
 #pragma unroll
@@ -60,18 +61,21 @@ __device__ __forceinline__ void scan3(int (&v)[3], int (*scratch)[3], long long 
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        int w = scratch[lane][k];                              // (32 warps)
+        int w = lane < PLAN_WARPS ? scratch[lane][k] : 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
+        for (int o = 1; o < PLAN_WARPS; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, w, o);
             if (lane >= o) w += u;
         }
         const int mine = warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
         before[k] = total[k] + mine + incl[k] - v[k];
-        total[k] += __shfl_sync(0xffffffffu, w, 31);
+        total[k] += __shfl_sync(0xffffffffu, w, PLAN_WARPS - 1);
     }
     __syncthreads();
 }
+
+// What the tokens are laid out by: where every request's begin, its row (-1: it has no pages in the step) and cached tokens.
+struct Known { int cu[PLAN_THREADS + 1], row[PLAN_THREADS], len[PLAN_THREADS]; };
 
 struct Request { int row, fresh, len, held, need, goes_to, goes, at; };   // (goes: pages [goes_to - goes, goes_to) go back)
 
@@ -87,9 +91,9 @@ __device__ __forceinline__ Request request_of(const LayoutParams& p, int s, bool
         r.need = p.free_pages ? 0 : r.held;
         r.goes_to = p.free_pages ? r.held : 0;
     } else {
-        const long long end = (long long)r.len + fresh, pages = (end + p.page_size - 1) / p.page_size;
-        ok = ok && r.len >= 0 && (long long)r.held * p.page_size >= r.len && end <= 0x7fffffffll && pages <= p.table_width && pages <= p.out_width &&
-             (p.free_pages || pages <= r.held) && fresh <= p.n_tokens && (!p.parents || fresh <= SPITE_MAX_DRAFTS) && (!p.ancestors || fresh <= 32 * p.n_words);
+        const unsigned end = (unsigned)r.len + (unsigned)fresh, pages = end / p.page_size + (end % p.page_size != 0);       // (len and fresh are below 2^31)
+        ok = ok && r.len >= 0 && (long long)r.held * p.page_size >= r.len && end <= 0x7fffffffu && pages <= (unsigned)min(p.table_width, p.out_width) &&
+             (p.free_pages || pages <= (unsigned)r.held) && fresh <= p.n_tokens && (!p.parents || fresh <= SPITE_MAX_DRAFTS) && (!p.ancestors || fresh <= 32 * p.n_words);
         r.need = ok ? max(r.held, (int)pages) : r.held;
         r.goes_to = ok && p.free_pages ? min(first_needed(p, r.len) / p.page_size, r.held) : 0;
     }
@@ -99,14 +103,12 @@ __device__ __forceinline__ Request request_of(const LayoutParams& p, int s, bool
 
 // One block plans the step and changes the persistent state: whose pages go back, who gets which.  A thread a request, a warp a
 // request where its pages are looked at.  The requests of a step are few and all it reads lies in L2, so that what counts is the
-// number of dependent reads; `plan` hands a request's row (-1: none) to the kernel that fills in the rest.
-__global__ void __launch_bounds__(PLAN_THREADS) layout_plan_kernel(const LayoutParams p, int* plan) {
+// number of dependent reads.  `known` (with no more requests than threads): filled in for what follows.
+__device__ void plan_step(const LayoutParams& p, Known* known) {
     extern __shared__ unsigned seen[];                         // a bit a row of the tables
     __shared__ Request reqs[PLAN_THREADS];
-    __shared__ int scratch[32][3];
+    __shared__ int scratch[PLAN_WARPS][3];
     __shared__ int bad;
-    pdl_wait();
-    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = (p.n_rows + 31) / 32;
     for (int i = threadIdx.x; i < words; i += PLAN_THREADS) seen[i] = 0;
     if (threadIdx.x == 0) bad = 0;
@@ -123,9 +125,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) layout_plan_kernel(const LayoutP
             if (check && ok && r.row >= 0) ok = (atomicOr(&seen[r.row / 32], 1u << (r.row % 32)) >> (r.row % 32) & 1u) == 0;
             if (!ok) { bad = SPITE_LAYOUT_MALFORMED; r.row = -1; }
         }
+        if (r.goes_to > 0 && p.tables[(size_t)r.row * p.table_width + r.goes_to - 1] < 0) r.goes_to = 0;     // (they have gone already)
         reqs[threadIdx.x] = r;
-        __syncthreads();
-        for (int i = warp; i < min(PLAN_THREADS, p.n_requests - s0); i += PLAN_THREADS / 32) {
+        if (!__syncthreads_or(r.goes_to)) return r;
+        for (int i = warp; i < min(PLAN_THREADS, p.n_requests - s0); i += PLAN_WARPS) {
             const Request q = reqs[i];
             if (q.row < 0 || q.goes_to == 0) continue;
             const int* table = p.tables + (size_t)q.row * p.table_width;
@@ -161,7 +164,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) layout_plan_kernel(const LayoutP
     }
     __syncthreads();
     if (bad) {                                                 // nothing is changed and the step has no tokens
-        for (int s = threadIdx.x; s < p.n_requests; s += PLAN_THREADS) { plan[s] = -1; p.cu_seqlens[s] = 0; }
+        for (int s = threadIdx.x; s < p.n_requests; s += PLAN_THREADS) p.cu_seqlens[s] = 0;
+        if (known) {
+            known->cu[threadIdx.x] = 0;
+            known->row[threadIdx.x] = -1;
+            if (threadIdx.x == 0) known->cu[PLAN_THREADS] = 0;
+        }
         return;
     }
     const int top = n_free + (int)total[1];                    // the stack's height once the pages are back
@@ -173,14 +181,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) layout_plan_kernel(const LayoutP
             scan3(v, scratch, run, before);
         }
         const int s = s0 + threadIdx.x;
-        if (s < p.n_requests) {
-            p.cu_seqlens[s] = (int)before[0];
-            plan[s] = r.row;
+        if (s < p.n_requests) p.cu_seqlens[s] = (int)before[0];
+        if (known) {
+            known->cu[threadIdx.x] = (int)before[0];           // (behind the last request: all tokens)
+            known->row[threadIdx.x] = r.fresh >= 0 ? r.row : -1;
+            known->len[threadIdx.x] = r.len;
+            if (threadIdx.x == 0) known->cu[PLAN_THREADS] = (int)total[0];
         }
         if (total[1] == 0) continue;                           // (the same for all)
         reqs[threadIdx.x].at = n_free + (int)before[1];
         __syncthreads();
-        for (int i = warp; i < min(PLAN_THREADS, p.n_requests - s0); i += PLAN_THREADS / 32) {
+        for (int i = warp; i < min(PLAN_THREADS, p.n_requests - s0); i += PLAN_WARPS) {
             const Request q = reqs[i];
             if (q.row < 0 || q.goes == 0) continue;
             int* table = p.tables + (size_t)q.row * p.table_width + q.goes_to - q.goes;
@@ -205,90 +216,168 @@ __global__ void __launch_bounds__(PLAN_THREADS) layout_plan_kernel(const LayoutP
             scan3(v, scratch, taken, before);
         }
         r.at = top - 1 - (int)before[2];
+        const int takes = r.row >= 0 ? r.need - r.held : 0;
+        int* mine = p.tables + (size_t)max(r.row, 0) * p.table_width + r.held;
+        for (int k = 0; k < min(takes, FEW_PAGES); ++k) mine[k] = p.free_pages[r.at - k];
+        if (takes) p.held[r.row] = r.need;                     // (an ended request's, to none)
         reqs[threadIdx.x] = r;
-        __syncthreads();
-        for (int i = warp; i < min(PLAN_THREADS, p.n_requests - s0); i += PLAN_THREADS / 32) {
+        if (!__syncthreads_or(takes > FEW_PAGES)) continue;    // a prompt's, by a warp each
+        for (int i = warp; i < min(PLAN_THREADS, p.n_requests - s0); i += PLAN_WARPS) {
             const Request q = reqs[i];
             if (q.row < 0) continue;
             int* table = p.tables + (size_t)q.row * p.table_width + q.held;
-            for (int k = lane; k < q.need - q.held; k += 32) table[k] = p.free_pages[q.at - k];
-            if (lane == 0) p.held[q.row] = q.need;
+            for (int k = FEW_PAGES + lane; k < q.need - q.held; k += 32) table[k] = p.free_pages[q.at - k];
         }
         __syncthreads();
     }
     if (threadIdx.x == 0) *p.n_free = top - (int)total[2];
 }
 
-// Everything that follows from the plan, a thread a number: grid (blocks over tokens, then over the block table's rows).
-__global__ void __launch_bounds__(256) layout_fill_kernel(const LayoutParams p, const int* plan, int token_blocks) {
+// Everything that follows from the plan, a thread a number, by `n` threads of which this is number `i`; `known` or, without it, what lies in global
+// memory, where the search through cu_seqlens is a chain of reads from L2.  (With a bad status the requests have no tokens and no pages.)
+__device__ void fill_step(const LayoutParams& p, const Known* known, bool bad, long long i, long long n) {
+    auto cu = [&](int s) { return known ? known->cu[s] : p.cu_seqlens[s]; };
+    auto row_of = [&](int s) { return known ? known->row[s] : !bad && p.slots[s] >= 0 && p.new_tokens[s] >= 0 ? p.slots[s] : -1; };
+    const long long total = bad ? 0 : cu(p.n_requests);
+    for (long long t = i; t < total; t += n) {
+        int lo = 0, hi = p.n_requests;                         // cu[lo] <= t < cu[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (cu(mid) <= t) lo = mid; else hi = mid;
+        }
+        const int row = row_of(lo), first = cu(lo), node = (int)t - first, len = known ? known->len[lo] : p.lengths[row], place = len + node;
+        bool real = true;
+        int depth = node;
+        if (p.parents) {
+            // A token's ancestors, from itself upward: the parents' numbers fall, so the words of its set are finished one by one.  (A parent
+            // that is not in front of its child ends the walk; one below -1 marks padding, which has no row in the cache.)
+            depth = 0;
+            real = p.parents[t] >= -1;
+            unsigned* set = p.ancestors ? p.ancestors + t * p.n_words : nullptr;
+            int word = p.n_words - 1, at = real ? node : -1;
+            unsigned bits = 0;
+            while (at >= 0) {
+                if (set) {
+                    for (; word > at / 32; --word) { set[word] = bits; bits = 0; }
+                    bits |= 1u << (at % 32);
+                }
+                const int up = p.parents[first + at];
+                if (up >= at || up < 0) break;
+                at = up;
+                ++depth;
+            }
+            if (set)
+                for (; word >= 0; --word) { set[word] = bits; bits = 0; }
+        } else if (p.ancestors) {
+            for (int w = 0; w < p.n_words; ++w)
+                p.ancestors[t * p.n_words + w] = w < node / 32 ? 0xffffffffu : w > node / 32 ? 0u : 0xffffffffu >> (31 - node % 32);
+        }
+        p.positions[t] = len + depth;
+        p.seg_of_token[t] = lo;
+        const int page = p.tables[(size_t)row * p.table_width + place / p.page_size];
+        p.slot_map[t] = real && page >= 0 ? (long long)page * p.page_size + place % p.page_size : -1;
+    }
+    // the block table, a warp a row (or several a row): the rows' addresses are then the same for its lanes
+    constexpr int AHEAD = 8;                                   // numbers of a lane asked for together
+    const int lane = (int)(i & 31), per = (p.out_width + 32 * AHEAD - 1) / (32 * AHEAD);
+    for (long long piece = i >> 5; piece < (long long)p.n_requests * per; piece += n >> 5) {
+        const int s = (int)((unsigned)piece / (unsigned)per), c0 = ((int)piece - s * per) * 32 * AHEAD + lane, row = row_of(s);
+        const bool has = row >= 0;
+        const int* from = p.tables + (size_t)(has ? row : 0) * p.table_width;
+        int* to = p.block_table + (size_t)s * p.out_width;
+        int v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) v[k] = has && c0 + 32 * k < min(p.table_width, p.out_width) ? from[c0 + 32 * k] : -1;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (c0 + 32 * k < p.out_width) to[c0 + 32 * k] = v[k];
+    }
+}
+
+// The whole in one launch, for up to PLAN_THREADS requests: one block, or a cluster of which the first block plans while the others look up what
+// does not depend on the plan and wait at the cluster's barrier.
+__global__ void __launch_bounds__(PLAN_THREADS) layout_kernel(const LayoutParams p) {
+    __shared__ Known known;
+    __shared__ int status;
     pdl_wait();
     pdl_launch_dependents();
-    if ((int)blockIdx.x >= token_blocks) {
-        const int per = (p.out_width + 255) / 256, b = blockIdx.x - token_blocks, s = b / per, col = (b % per) * 256 + threadIdx.x;
-        const int row = plan[s];
-        if (col < p.out_width) {
-            const bool ended = row >= 0 && p.new_tokens[s] < 0;
-            p.block_table[(size_t)s * p.out_width + col] = row >= 0 && !ended && col < p.table_width ? p.tables[(size_t)row * p.table_width + col] : -1;
-        }
-        return;
+    if (blockIdx.x == 0) {
+        plan_step(p, &known);
+    } else if ((int)threadIdx.x < p.n_requests) {
+        const int row = p.slots[threadIdx.x];
+        const bool has = row >= 0 && row < p.n_rows && p.new_tokens[threadIdx.x] >= 0;
+        known.row[threadIdx.x] = has ? row : -1;
+        known.len[threadIdx.x] = has ? p.lengths[row] : 0;
     }
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= p.cu_seqlens[p.n_requests]) return;
-    int lo = 0, hi = p.n_requests;                             // cu[lo] <= t < cu[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu_seqlens[mid] <= t) lo = mid; else hi = mid;
+    if (gridDim.x > 1) {
+        __threadfence();
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (blockIdx.x != 0)
+            for (int s = threadIdx.x; s <= p.n_requests; s += PLAN_THREADS) known.cu[s] = __ldcg(p.cu_seqlens + s);
     }
-    const int row = plan[lo], first = p.cu_seqlens[lo], node = t - first, len = p.lengths[row], place = len + node;
-    bool real = true;
-    int depth = node;
-    if (p.parents) {
-        // A token's ancestors, from itself upward: the parents' numbers fall, so the words of its set are finished one by one.  (A parent
-        // that is not in front of its child ends the walk; one below -1 marks padding, which has no row in the cache.)
-        depth = 0;
-        real = p.parents[t] >= -1;
-        unsigned* set = p.ancestors ? p.ancestors + (size_t)t * p.n_words : nullptr;
-        int word = p.n_words - 1, at = real ? node : -1;
-        unsigned bits = 0;
-        while (at >= 0) {
-            if (set) {
-                for (; word > at / 32; --word) { set[word] = bits; bits = 0; }
-                bits |= 1u << (at % 32);
-            }
-            const int up = p.parents[first + at];
-            if (up >= at || up < 0) break;
-            at = up;
-            ++depth;
-        }
-        if (set)
-            for (; word >= 0; --word) { set[word] = bits; bits = 0; }
-    } else if (p.ancestors) {
-        for (int w = 0; w < p.n_words; ++w)
-            p.ancestors[(size_t)t * p.n_words + w] = w < node / 32 ? 0xffffffffu : w > node / 32 ? 0u : 0xffffffffu >> (31 - node % 32);
+    if (threadIdx.x == 0) status = __ldcg(p.status);
+    __syncthreads();
+    const bool bad = status != 0;
+    if (bad && (int)threadIdx.x < p.n_requests) known.row[threadIdx.x] = -1;
+    __syncthreads();
+    fill_step(p, &known, bad, (long long)blockIdx.x * PLAN_THREADS + threadIdx.x, (long long)gridDim.x * PLAN_THREADS);
+}
+// In two: the plan, and as many blocks as a large table needs.
+__global__ void __launch_bounds__(PLAN_THREADS) layout_plan_kernel(const LayoutParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    plan_step(p, nullptr);
+}
+__global__ void __launch_bounds__(256) layout_fill_kernel(const LayoutParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    fill_step(p, nullptr, *p.status != 0, (long long)blockIdx.x * 256 + threadIdx.x, (long long)gridDim.x * 256);
+}
+
+// A launch of one cluster (of one block: an ordinary one).
+void launch_cluster(const LayoutParams& p, int blocks, size_t smem, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (spite_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
     }
-    p.positions[t] = len + depth;
-    p.seg_of_token[t] = lo;
-    const int page = p.tables[(size_t)row * p.table_width + place / p.page_size];
-    p.slot_map[t] = real && page >= 0 ? (long long)page * p.page_size + place % p.page_size : -1;
+    if (blocks > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = blocks;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    (void)cudaLaunchKernelEx(&cfg, layout_kernel, p);
 }
 
 }  // namespace
 
-// Lays a step out.  `plan`: n_requests ints of scratch.
-SPITE_API int spite_layout_step(const LayoutParams* p, int* plan, void* stream) {
-    if (!p || !plan || !p->tables || !p->held || !p->slots || !p->lengths || !p->new_tokens || !p->block_table || !p->cu_seqlens || !p->status)
-        return SPITE_BAD_ARG;
+// Lays a step out.  `blocks`: one launch of a cluster of so many (1..8), for up to 512 requests, or 0: two launches.
+SPITE_API int spite_layout_step(const LayoutParams* p, int blocks, void* stream) {
+    if (!p || !p->tables || !p->held || !p->slots || !p->lengths || !p->new_tokens || !p->block_table || !p->cu_seqlens || !p->status) return SPITE_BAD_ARG;
     if (!p->free_pages != !p->n_free || p->n_rows < 1 || p->table_width < 1 || p->out_width < 1 || p->n_requests < 1 || p->page_size < 1) return SPITE_BAD_ARG;
     if (p->n_tokens < 0 || (p->n_tokens > 0 && (!p->positions || !p->seg_of_token || !p->slot_map))) return SPITE_BAD_ARG;
     if (p->window_kind < 0 || p->window_kind > 2 || (p->window_kind && p->window_size < 1)) return SPITE_BAD_ARG;
-    if ((p->ancestors && p->n_words < 1) || (p->free_pages && p->n_pages < 1) || (p->parents && p->n_parents < 0)) return SPITE_BAD_ARG;
-    if (p->n_tokens > (1 << 20) || p->table_width > (1 << 20) || p->n_requests > SPITE_LAYOUT_MAX_REQUESTS || p->n_rows > SPITE_LAYOUT_MAX_ROWS || p->n_words > SPITE_MAX_DRAFTS / 32) return SPITE_UNSUPPORTED;
+    if ((p->ancestors && p->n_words < 1) || (p->free_pages && p->n_pages < 1) || (p->parents && p->n_parents < 0) || blocks < 0 || blocks > 8) return SPITE_BAD_ARG;
+    if (p->n_tokens > (1 << 20) || p->table_width > (1 << 20) || p->n_requests > SPITE_LAYOUT_MAX_REQUESTS || p->n_rows > SPITE_LAYOUT_MAX_ROWS ||
+        p->n_words > SPITE_MAX_DRAFTS / 32 || (blocks && p->n_requests > PLAN_THREADS)) return SPITE_UNSUPPORTED;
     cudaStream_t st = (cudaStream_t)stream;
-    SPITE_LAUNCH(layout_plan_kernel, 1, PLAN_THREADS, (size_t)(p->n_rows + 31) / 32 * 4, st, *p, plan);
-    const int token_blocks = (p->n_tokens + 255) / 256;
-    const long long blocks = token_blocks + (long long)p->n_requests * ((p->out_width + 255) / 256);
-    if (blocks > 0x7fffffffll) return SPITE_UNSUPPORTED;
-    SPITE_LAUNCH(layout_fill_kernel, (unsigned)blocks, 256, 0, st, *p, (const int*)plan, token_blocks);
+    const size_t smem = (size_t)(p->n_rows + 31) / 32 * 4;
+    if (blocks) {
+        launch_cluster(*p, blocks, smem, st);
+    } else {
+        SPITE_LAUNCH(layout_plan_kernel, 1, PLAN_THREADS, smem, st, *p);
+        const long long pieces = (long long)p->n_requests * ((p->out_width + 255) / 256), fill = (pieces + 7) / 8;
+        SPITE_LAUNCH(layout_fill_kernel, (unsigned)(fill < 2048 ? fill : 2048), 256, 0, st, *p);
+    }
     return spite_launch_status();
 }
 

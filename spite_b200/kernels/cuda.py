@@ -348,6 +348,10 @@ class CudaKernels(KernelSet):
         # most key splits of decode attention: beyond about twenty the merge by the last block costs more than the
         # extra blocks bring (one request at 8,192 keys: 22 us with 37 splits, 17.6 us with 18)
         self.attention_max_splits = 24
+        # numbers that `layout_step` writes up to which it is one block, then one cluster of eight blocks, else two launches.  us on the device, one /
+        # cluster / two: 64 words 5.2 / 5.7 / 6.4, 4,160 6.3 / 6.5 / 7.6, 65,000 17 / 7.4 / 7.6, 131,136 20 / 8.6 / 8.1, 265,000 42 / 11 / 8.4;
+        # a launch takes the host 2.5
+        self.layout_words = (1 << 13, 160_000)
         self.attention_narrow_rows = 8         # decoded tokens of up to so many heads a kv head take its form of eight rows (0: never)
         self.use_decode_attention = True       # the TMA-fed decode kernel (head sizes 64 and 128, pages of a multiple of 64 keys)
         # row counts up to which the weight-streaming kernel is preferred over the tcgen05 one
@@ -1252,17 +1256,13 @@ class CudaKernels(KernelSet):
             f.argtypes = argtypes
         return f
 
-    def _whole_numbers(self, what, tensors, dtype=torch.int32):
-        """`tensors`: (name, tensor, dimensions), contiguous tensors of `dtype` on the device."""
-        for name, t, dims in tensors:
-            if not (t.is_cuda and t.is_contiguous() and t.dtype is dtype and t.dim() == dims):
-                raise KernelError(f"{what}: {name} must be a contiguous CUDA tensor of {dtype} with {dims} dimensions")
-
-    def _on_current_device(self, what, t) -> int:
-        """The current stream's handle; the launch goes to the current device, which has to be the tensors'."""
-        if t.get_device() != torch.cuda.current_device():
-            raise KernelError(f"{what}: the tensors are on {t.device}, the current device is another")
-        return self._raw_stream()
+    @staticmethod
+    def _whole_numbers(what, device, names, tensors, dims, dtype=torch.int32):
+        """`tensors` (`names`, for the message): contiguous, of `dtype`, with `dims` dimensions, on the current device, which is where the launch goes."""
+        for t in tensors:
+            if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or t.dim() != dims:
+                raise KernelError(f"{what}: {names} must be contiguous {dtype} tensors with {dims} dimension(s) on the current device, cuda:{device}; "
+                                  f"one is {t.dtype}, {tuple(t.shape)}, on {t.device}")
 
     def tree_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, sink_logit=None, head_sinks=None, head_slopes=None,
                        head_gates=None, out_by_head=False, score_softcap=None, distance_bias=None):
@@ -1271,7 +1271,9 @@ class CudaKernels(KernelSet):
         M, table, cu, positions, seg, sets = batch.n_tokens, batch.block_tables[cache.group], batch.cu_seqlens, batch.positions, batch.seg_of_token, batch.ancestors
         if sets is None:
             raise KernelError(f"{what}: the step has no ancestor sets")
-        self._whole_numbers(what, (("positions", positions, 1), ("seg_of_token", seg, 1), ("cu_seqlens", cu, 1), ("block_table", table, 2), ("ancestors", sets, 2)))
+        device = torch.cuda.current_device()
+        self._whole_numbers(what, device, "positions, seg_of_token and cu_seqlens", (positions, seg, cu), 1)
+        self._whole_numbers(what, device, "block_table and ancestors", (table, sets), 2)
         kv, scales = cache.kv, cache.key_scale
         self._t(kv, self.dtype, "cache")
         planes, n_pages, kv_heads, page, hd = kv.shape
@@ -1286,7 +1288,9 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: heads of {hd} elements; up to 256 are supported")
         if not M:
             return
-        stream = self._on_current_device(what, q)
+        if q.get_device() != device:
+            raise KernelError(f"{what}: q is on {q.device}, the current device is cuda:{device}")
+        stream = self._raw_stream()
         has_sink = sink_logit is not None or head_sinks is not None
         call = _TREE_CALL.pack(
             q.data_ptr(), out.data_ptr(), num_heads, _WINDOW[window.kind], window.size, softmax_scale, has_sink, sink_logit or 0.0,
@@ -1324,59 +1328,58 @@ class CudaKernels(KernelSet):
     # ------------------------------------------------------------------ steps laid out and drafts accepted on the device
     def layout_step(self, pages, slots, lengths, new_tokens, out, *, parents=None):
         what, tables, held, free, n_free = "layout_step", pages.tables, pages.held, pages.free_pages, pages.n_free
-        block, cu, positions, seg, sets, status = out.block_table, out.cu_seqlens, out.positions, out.seg_of_token, out.ancestors, out.status
-        self._whole_numbers(what, (("tables", tables, 2), ("held", held, 1), ("slots", slots, 1), ("lengths", lengths, 1), ("new_tokens", new_tokens, 1),
-                                   ("block_table", block, 2), ("cu_seqlens", cu, 1), ("positions", positions, 1), ("seg_of_token", seg, 1), ("status", status, 1)))
-        self._whole_numbers(what, (("slot_map", out.slot_map, 1),), torch.int64)
+        block, cu, positions, seg, sets, status, slot_map = out.block_table, out.cu_seqlens, out.positions, out.seg_of_token, out.ancestors, out.status, out.slot_map
         if (free is None) != (n_free is None):
             raise KernelError(f"{what}: a stack of free pages needs its height, and the other way round")
+        device = torch.cuda.current_device()
+        self._whole_numbers(what, device, "tables, block_table and ancestors", (tables, block) if sets is None else (tables, block, sets), 2)
+        self._whole_numbers(what, device, "held, slots, lengths, new_tokens, cu_seqlens, positions, seg_of_token and status",
+                            (held, slots, lengths, new_tokens, cu, positions, seg, status), 1)
+        self._whole_numbers(what, device, "slot_map", (slot_map,), 1, torch.int64)
         if free is not None:
-            self._whole_numbers(what, (("free_pages", free, 1), ("n_free", n_free, 1)))
+            self._whole_numbers(what, device, "free_pages and n_free", (free, n_free), 1)
         if parents is not None:
-            self._whole_numbers(what, (("parents", parents, 1),))
-        if sets is not None:
-            self._whole_numbers(what, (("ancestors", sets, 2),))
+            self._whole_numbers(what, device, "parents", (parents,), 1)
         S, (R, W), M, (block_rows, out_width) = slots.numel(), tables.shape, positions.numel(), block.shape
         n_sets, n_words = (M, 0) if sets is None else sets.shape
         if held.numel() != R or lengths.numel() != R or new_tokens.numel() != S or block_rows != S or cu.numel() != S + 1:
             raise KernelError(f"{what}: {S} requests in {R} rows: held and lengths have a number a row, new_tokens and block_table one a request, cu_seqlens one more")
-        if seg.numel() != M or out.slot_map.numel() != M or n_sets != M:
+        if seg.numel() != M or slot_map.numel() != M or n_sets != M:
             raise KernelError(f"{what}: positions, seg_of_token, slot_map and ancestors have room for the same number of tokens")
         if status.numel() != 1 or (n_free is not None and n_free.numel() != 1):
             raise KernelError(f"{what}: status and n_free are one number each")
         if not S or not W or not out_width or pages.page_size < 1 or (sets is not None and not n_words):
             raise KernelError(f"{what}: a step needs requests, and pages, tables and sets that are not empty")
-        stream = self._on_current_device(what, slots)
-        plan = torch.empty(S, dtype=torch.int32, device=slots.device)
         call = _LAYOUT_CALL.pack(
             tables.data_ptr(), held.data_ptr(), _address(free), _address(n_free), slots.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), _address(parents),
-            block.data_ptr(), cu.data_ptr(), positions.data_ptr(), seg.data_ptr(), out.slot_map.data_ptr(), _address(sets), status.data_ptr(),
+            block.data_ptr(), cu.data_ptr(), positions.data_ptr(), seg.data_ptr(), slot_map.data_ptr(), _address(sets), status.data_ptr(),
             R, W, 0 if free is None else free.numel(), S, out_width, M, 0 if parents is None else parents.numel(), n_words, pages.page_size,
             _WINDOW[pages.window.kind], pages.window.size)
-        st = self._entry("drafts", "spite_layout_step", C.c_char_p, C.c_void_p, C.c_void_p)(call, plan.data_ptr(), stream)
-        self._count("drafts", 2)
+        # one block while there is little to write, then a cluster of eight, then two launches (see `layout_words`)
+        words = S * out_width + M * (4 + n_words)
+        blocks = 0 if S > 512 or words > self.layout_words[1] else 1 if words <= self.layout_words[0] else 8
+        st = self._entry("drafts", "spite_layout_step", C.c_char_p, C.c_int, C.c_void_p)(call, blocks, self._raw_stream())
+        self._count("drafts", 1 if blocks else 2)
         _check(st, what)
 
     def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
-        what = "accept_drafts"
-        self._whole_numbers(what, (("tokens", tokens, 1), ("targets", targets, 1), ("cu_seqlens", cu_seqlens, 1), ("counts", counts, 1), ("path", path, 2),
-                                   ("emitted", emitted, 2)))
+        what, device = "accept_drafts", torch.cuda.current_device()
+        self._whole_numbers(what, device, "tokens, targets, cu_seqlens and counts", (tokens, targets, cu_seqlens, counts), 1)
+        self._whole_numbers(what, device, "path and emitted", (path, emitted), 2)
+        for name, t in (("parents", parents), ("slots", slots), ("lengths", lengths), ("lengths_out", lengths_out)):
+            if t is not None:
+                self._whole_numbers(what, device, name, (t,), 1)
         S, M, (rows, depth) = cu_seqlens.numel() - 1, tokens.numel(), path.shape
-        if parents is not None:
-            self._whole_numbers(what, (("parents", parents, 1),))
         if targets.numel() != M or (parents is not None and parents.numel() != M):
             raise KernelError(f"{what}: {M} tokens have a parent and a target each")
         if S < 1 or counts.numel() != S or rows != S or not depth or emitted.shape != path.shape:
             raise KernelError(f"{what}: {S} requests: counts has a number, path and emitted a row of the same length for each")
         if (lengths is None) != (lengths_out is None):
             raise KernelError(f"{what}: lengths and lengths_out go together")
-        if slots is not None:
-            self._whole_numbers(what, (("slots", slots, 1),))
-            if slots.numel() != S:
-                raise KernelError(f"{what}: {slots.numel()} slots for {S} requests")
+        if slots is not None and slots.numel() != S:
+            raise KernelError(f"{what}: {slots.numel()} slots for {S} requests")
         n_rows = 0
         if lengths is not None:
-            self._whole_numbers(what, (("lengths", lengths, 1), ("lengths_out", lengths_out, 1)))
             n_rows = lengths.numel()
             if n_rows != lengths_out.numel() or (slots is None and n_rows < S):
                 raise KernelError(f"{what}: lengths and lengths_out have a number a row")
@@ -1386,7 +1389,7 @@ class CudaKernels(KernelSet):
         for kv, slot_map, scales in caches:
             if self._t(kv, self.dtype, f"{what}: cache").dim() != 6 or not kv.numel():
                 raise KernelError(f"{what}: a cache is [caches, planes, pages, kv heads, page_size, head_dim]")
-            self._whole_numbers(what, (("slot_map", slot_map, 1),), torch.int64)
+            self._whole_numbers(what, device, "slot_map", (slot_map,), 1, torch.int64)
             if slot_map.numel() < M:
                 raise KernelError(f"{what}: the slot map has {slot_map.numel()} rows for {M} tokens")
             n, planes, n_pages, heads, page, size = kv.shape
@@ -1396,13 +1399,12 @@ class CudaKernels(KernelSet):
             groups.append(_ACCEPT_GROUP.pack(kv.data_ptr(), _address(scales), slot_map.data_ptr(), n_pages * heads * page * row_bytes, n * planes, n, n_pages,
                                              heads, page, row_bytes))
             most = max(most, n * planes * heads * row_bytes // 16)
-        stream = self._on_current_device(what, tokens)
         call = _ACCEPT_CALL.pack(tokens.data_ptr(), _address(parents), targets.data_ptr(), cu_seqlens.data_ptr(), counts.data_ptr(), path.data_ptr(),
                                  emitted.data_ptr(), _address(slots), _address(lengths), _address(lengths_out), M, S, depth, n_rows, len(groups),
                                  b"".join(groups))
         # a thread for every 16 bytes of a token's rows, as long as that is not far more blocks than the device holds
         pieces = max(1, min(-(-most // 256), max(1, 16 * self.sm_count // S)))
-        st = self._entry("drafts", "spite_accept_drafts", C.c_char_p, C.c_int, C.c_void_p)(call, pieces, stream)
+        st = self._entry("drafts", "spite_accept_drafts", C.c_char_p, C.c_int, C.c_void_p)(call, pieces, self._raw_stream())
         self._count("drafts", 1)
         _check(st, what)
 
