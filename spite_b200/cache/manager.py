@@ -254,22 +254,31 @@ class CacheManager:
             rc.pending[g] = []
         rc.reserved = 0
 
-    def commit(self, req_id) -> list[list[int]]:
-        """The step ran: the reserved tokens are cached.  Pages that every later
-        token's window has passed are freed; returns them per group."""
+    def commit(self, req_id, kept: int | None = None) -> list[list[int]]:
+        """The step ran: the reserved tokens are cached, or the first `kept` of them (the others were drafts that were not accepted).  Pages
+        that every later token's window has passed are freed, and those that hold none of the kept tokens; returns them per group."""
         rc = self.get(req_id)
         if not rc.reserved:
             raise CacheError(f"request {req_id!r} has nothing reserved")
-        rc.n_tokens += rc.reserved
+        if kept is None:
+            kept = rc.reserved
+        if not 0 <= kept <= rc.reserved:
+            raise CacheError(f"request {req_id!r}: {kept} tokens kept of {rc.reserved}")
+        rc.n_tokens += kept
         rc.reserved = 0
         rc.fresh = False
         freed = []
         for g, key in enumerate(self.groups):
             rc.pending[g] = []
-            rc.len_before[g] = len(rc.tables[g])
             first_live = key.window.first_needed(rc.n_tokens) // self.page_size
             out = []
             table = rc.tables[g]
+            while len(table) > -(-rc.n_tokens // self.page_size):
+                page = table.pop()
+                if page >= 0:
+                    self.pools[g].free(page)
+                    out.append(page)
+            rc.len_before[g] = len(table)
             for lp in range(min(first_live, len(table))):
                 if table[lp] >= 0:
                     self.pools[g].free(table[lp])

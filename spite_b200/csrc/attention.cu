@@ -43,8 +43,11 @@ __global__ void __launch_bounds__(256) qk_prepare_kernel(const QkPrepareParams p
         for (int h = threadIdx.x; h < nq; h += blockDim.x)
             p.gates_out[(size_t)t * nq + h] =
                 1.0f / (1.0f + expf(-to_f32(((const T*)p.qkv)[(size_t)t * p.qkv_stride + (size_t)heads_total * hd + h])));
-    int page = -1;
-    if (p.write_cache && !p.q_only) {
+    int page = -1, place = pos % c.page_size;
+    if (p.write_cache && !p.q_only && p.slot_map) {
+        const long long slot = p.slot_map[t];
+        if (slot >= 0 && slot < (long long)c.n_pages * c.page_size) { page = (int)(slot / c.page_size); place = (int)(slot % c.page_size); }
+    } else if (p.write_cache && !p.q_only) {
         page = b.block_table[(size_t)b.seg_of_token[t] * b.table_width + pos / c.page_size];
         if (page >= c.n_pages) page = -1;                     // the host never lets this happen
         // A captured step pads its rows with copies of its first row.  Behind a recurrent layer a copy's row is not the
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(256) qk_prepare_kernel(const QkPrepareParams p
             if (page < 0) continue;                          // nothing to append (or no page: the host never lets this happen)
             const int kvh = is_v ? head - nq - nkv : head - nq;
             dst = (T*)c.kv + (is_v ? c.v_offset : 0) +
-                  (((size_t)page * nkv + kvh) * c.page_size + pos % c.page_size) * hd;
+                  (((size_t)page * nkv + kvh) * c.page_size + place) * hd;
         }
         const float* bias = p.bias ? p.bias + (size_t)head * hd : nullptr;
         if (is_v) {
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(256) qk_prepare_kernel(const QkPrepareParams p
             }
             ss = warp_sum(ss);
             if (lane == 0)
-                c.key_scale[((size_t)page * nkv + head - nq) * c.page_size + pos % c.page_size] =
+                c.key_scale[((size_t)page * nkv + head - nq) * c.page_size + place] =
                     norm ? 1.0f / sqrtf(ss / norm_n + p.qk_norm_eps) : 1.0f;
             continue;
         }
@@ -221,8 +224,11 @@ __global__ void __launch_bounds__(256) qk_prepare_vec_kernel(const QkPreparePara
         raw[it] = head < heads_total ? *(const uint4*)(row + (size_t)head * HD + 8 * l) : make_uint4(0, 0, 0, 0);
     }
     const int pos = b.positions[t];
-    int page = -1;
-    if (p.write_cache && !p.q_only) {
+    int page = -1, place = pos % c.page_size;
+    if (p.write_cache && !p.q_only && p.slot_map) {
+        const long long slot = p.slot_map[t];
+        if (slot >= 0 && slot < (long long)c.n_pages * c.page_size) { page = (int)(slot / c.page_size); place = (int)(slot % c.page_size); }
+    } else if (p.write_cache && !p.q_only) {
         const int at = pos / c.page_size;
         page = b.block_table[(size_t)b.seg_of_token[t] * b.table_width + at];
         if (page >= c.n_pages) page = -1;                     // the host never lets this happen
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(256) qk_prepare_vec_kernel(const QkPreparePara
         if (is_q) dst = (__nv_bfloat16*)p.q_out + ((size_t)t * nq + head) * HD;
         else
             dst = (__nv_bfloat16*)c.kv + (is_v ? c.v_offset : 0) +
-                  (((size_t)page * nkv + (is_v ? head - nq - nkv : head - nq)) * c.page_size + pos % c.page_size) * HD;
+                  (((size_t)page * nkv + (is_v ? head - nq - nkv : head - nq)) * c.page_size + place) * HD;
         unsigned w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

@@ -77,6 +77,9 @@ struct QkPrepareParams {
     // the values are the projected keys (bias included): a row of qkv holds q heads and k heads alone, a cache of one plane
     // takes the keys as projected, and what the norm would multiply a key by goes to the cache's key_scale
     int values_are_keys;
+    // the row of the cache (page * page_size + place in it, or -1: none) that token t's key and value go to, or null: the row of its position (a
+    // step of drafted trees, whose nodes lie one behind the other in the cache while their positions are depths)
+    const long long* slot_map;
 };
 
 // cos and sin of pos * (freq + low).  With `low` the product's own rounding error and the frequency's are put back to second

@@ -1,7 +1,7 @@
 from .batch import Segment, StepBatch, build_step_batch
-from .executor import ContextOverflow, Engine, StepEntry, StepError
+from .executor import ContextOverflow, DraftTree, Engine, StepEntry, StepError
 from ..kernels.api import KernelTimeout
 from .model import Model, resolve_dtype
 
-__all__ = ["Segment", "StepBatch", "build_step_batch", "ContextOverflow", "Engine", "StepEntry",
+__all__ = ["Segment", "StepBatch", "build_step_batch", "ContextOverflow", "DraftTree", "Engine", "StepEntry",
            "StepError", "KernelTimeout", "Model", "resolve_dtype"]

@@ -97,6 +97,46 @@ def build_step_batch(segments, tokens_per_segment, wants, tables_per_group, devi
         max_seg_len=max((len(t) for t in tokens_per_segment), default=0))
 
 
+@dataclass
+class TreeBatch:
+    """What a step that verifies drafted trees brings besides its `StepBatch`: integers on the device, in one transfer."""
+    tokens: torch.Tensor           # [M] int32
+    parents: torch.Tensor          # [M] int32: number within the request, -1: none
+    slots: torch.Tensor            # [S] int32: 0 .. S - 1, the rows of what follows
+    lengths: torch.Tensor          # [S] int32: tokens cached
+    new_tokens: torch.Tensor       # [S] int32: nodes
+    tables: list                   # per group: [S, W] int32
+    held: list                     # per group: [S] int32
+
+
+def build_tree_batch(lengths, trees, tables_per_group, device, pin=True) -> TreeBatch:
+    """`trees[s]` = (tokens, parents) of request s, `tables_per_group[g][s]` its block table in group g, which reaches over its nodes."""
+    S, M = len(trees), sum(len(t) for t, _ in trees)
+    widths = [max(1, max(len(t) for t in tabs)) for tabs in tables_per_group]
+    host = torch.empty(2 * M + 3 * S + sum(S * (w + 1) for w in widths), dtype=torch.int32)
+    if pin and torch.device(device).type == "cuda":
+        host = host.pin_memory()
+    buf, o = host.numpy(), 0
+    places = []
+
+    def put(values):
+        nonlocal o
+        buf[o:o + len(values)] = values
+        places.append((o, len(values)))
+        o += len(values)
+    put([t for tokens, _ in trees for t in tokens])
+    put([p for _, parents in trees for p in parents])
+    put(range(S))
+    put(lengths)
+    put([len(t) for t, _ in trees])
+    for w, tabs in zip(widths, tables_per_group):
+        put([p for t in tabs for p in list(t) + [-1] * (w - len(t))])
+        put([len(t) for t in tabs])
+    dev = host.to(device, non_blocking=True)
+    views = [dev[a:a + n] for a, n in places]
+    return TreeBatch(*views[:5], tables=[views[5 + 2 * g].view(S, w) for g, w in enumerate(widths)], held=[views[6 + 2 * g] for g in range(len(widths))])
+
+
 class StaticDecodeBatch:
     """The inputs of a decode step (one token per request) at fixed device addresses,
     so that the step's kernels can be captured once in a CUDA graph and replayed:

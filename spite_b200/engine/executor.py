@@ -18,8 +18,10 @@ from dataclasses import dataclass
 import torch
 
 from ..cache import CacheError, CacheStorage, OutOfPages, OutOfSlots
-from ..kernels.api import KernelTimeout
-from .batch import Segment, StaticDecodeBatch, build_step_batch
+from ..kernels import build as kernel_build
+from ..kernels.api import KernelTimeout, PageTables, StepLayout
+from ..parts.base import Mixer
+from .batch import Segment, StaticDecodeBatch, StepBatch, build_step_batch, build_tree_batch
 
 
 class StepError(ValueError):
@@ -41,7 +43,18 @@ class StepEntry:
     want: list          # indices into `tokens` whose logits are asked for
 
 
+@dataclass
+class DraftTree:
+    """A request's next token and what may follow it: node 0 is the token that an ordinary step would bring, the others are drafted.
+    parents[i] < i is the number of the node that node i follows (parents[0] = -1); the same node may have several."""
+    req_id: object
+    tokens: list
+    parents: list
+
+
 class Engine:
+    MAX_DRAFTS = 1024           # nodes of a tree
+
     def __init__(self, model, *, cache_tokens: int, page_size: int = 64, max_requests: int = 64,
                  max_positions: int | None = None, cuda_graphs: bool | None = None, max_graphs: int = 32):
         if page_size < 1:
@@ -190,6 +203,92 @@ class Engine:
         self.steps_run += 1
         self.tokens_run += offset
         return logits
+
+    # ------------------------------------------------------------------ drafted tokens
+    def verify(self, trees, targets=None) -> list[list[int]]:
+        """Run one step over drafted trees (`DraftTree`s, one a request) and keep what the model agrees with.  Every node attends to its request's
+        cached tokens and to its ancestors; `targets(logits)` (float32 [nodes of all trees, vocab], tree by tree) gives the token that follows each
+        node, int32 [nodes] (default: the argmax, as in greedy decoding).  From node 0 the way goes to the child that is its node's target, as far
+        as there is one.  Returns for every request the targets along its way, which are the next tokens that single steps would have produced (as many as
+        nodes on the way, at least one); all of them but the last are cached then, like the tree's root, and the last is the next step's first
+        token.  The other nodes leave nothing behind.  Nothing is changed if the step cannot run."""
+        trees = [t if isinstance(t, DraftTree) else DraftTree(*t) for t in trees]
+        self.check()
+        if not all(part.follows_trees for _, part in self.model.parts() if isinstance(part, Mixer)):
+            raise StepError("drafted trees need layers without a state per request: one of the model's mixers keeps one")
+        vocab, seen = self.model.plan.vocab_size, set()
+        for t in trees:
+            n = len(t.tokens)
+            if t.req_id in seen:
+                raise StepError(f"request {t.req_id!r} appears twice in one step")
+            seen.add(t.req_id)
+            if not 1 <= n <= self.MAX_DRAFTS or len(t.parents) != n:
+                raise StepError(f"request {t.req_id!r}: a tree has 1 to {self.MAX_DRAFTS} tokens with a parent each, not {n} and {len(t.parents)}")
+            if t.parents[0] != -1 or any(not 0 <= int(p) < i for i, p in enumerate(t.parents) if i):
+                raise StepError(f"request {t.req_id!r}: parents[0] is -1, every other node's parent comes before it")
+            for tok in t.tokens:
+                if not 0 <= int(tok) < vocab:
+                    raise StepError(f"request {t.req_id!r}: token id {tok} outside the vocabulary of {vocab}")
+            have = self.cache.requests[t.req_id].n_tokens if t.req_id in self.cache.requests else 0
+            if have + n > self.max_positions:
+                raise ContextOverflow(f"request {t.req_id!r}: {have} cached + {n} drafted tokens exceed the limit of {self.max_positions} positions")
+        if not trees:
+            return []
+        kernels, device, storage = self.model.kernels, self.model.device, self.storage
+        if device.type == "cuda":
+            kernel_build.ensure_built(("attention_tree", "attention_tree_tc", "drafts", "sampling"))
+        admitted, reserved = [], []
+        try:
+            for t in trees:
+                if t.req_id not in self.cache.requests:
+                    self.cache.admit(t.req_id)
+                    admitted.append(t.req_id)
+            for t in trees:
+                self.cache.reserve(t.req_id, len(t.tokens))
+                reserved.append(t.req_id)
+            fresh_pages = [[p for t in trees for p in self.cache.pending_pages(t.req_id)[g]] for g in range(storage.n_groups)]
+            storage.clear_pages(kernels, fresh_pages)
+            held = [self.cache.requests[t.req_id] for t in trees]
+            step = build_tree_batch([rc.n_tokens for rc in held], [(t.tokens, t.parents) for t in trees],
+                                    [[rc.tables[g] for rc in held] for g in range(storage.n_groups)], device)
+            S, M = len(trees), step.tokens.numel()
+            ints = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=device)
+            layouts = []
+            for g, key in enumerate(storage.group_keys):
+                out = StepLayout(block_table=ints(S, step.tables[g].shape[1]), cu_seqlens=ints(S + 1), positions=ints(M), seg_of_token=ints(M),
+                                 slot_map=ints(M, dtype=torch.int64), status=ints(1), ancestors=ints(M, -(-max(len(t.tokens) for t in trees) // 32)))
+                kernels.layout_step(PageTables(step.tables[g], step.held[g], self.page_size, key.window), step.slots, step.lengths, step.new_tokens, out,
+                                    parents=step.parents)
+                layouts.append(out)
+            if not layouts:
+                raise StepError("drafted trees need a cache of keys and values: the model has none")
+            first = layouts[0]
+            batch = StepBatch(n_tokens=M, segments=[], token_ids=step.tokens, positions=first.positions, seg_of_token=first.seg_of_token,
+                              cu_seqlens=first.cu_seqlens, slots=step.slots, logit_rows=torch.arange(M, dtype=torch.int32, device=device),
+                              block_tables=[x.block_table for x in layouts], max_seg_len=max(len(t.tokens) for t in trees),
+                              ancestors=first.ancestors, slot_maps=[x.slot_map for x in layouts])
+            logits = self.model.forward(batch, storage)
+            chosen = kernels.argmax(logits) if targets is None else targets(logits)
+            depth = max(len(t.tokens) for t in trees)
+            counts, path, emitted = ints(S), ints(S, depth), ints(S, depth)
+            caches = [(storage.kv[g], layouts[g].slot_map, storage.key_scales[g]) for g in range(storage.n_groups)]
+            for g0 in range(0, len(caches), 8):              # (a call takes eight groups of caches)
+                kernels.accept_drafts(step.tokens, step.parents, chosen, first.cu_seqlens, caches[g0:g0 + 8], counts=counts, path=path, emitted=emitted)
+            result = torch.cat([counts[:, None], emitted, torch.stack([x.status for x in layouts], 1).expand(S, -1)], 1).tolist()
+            self.check()
+            if any(row[1 + depth:] != [0] * len(layouts) for row in result):
+                raise CacheError(f"the step's tables could not be laid out: status {result[0][1 + depth:]}")
+        except Exception:
+            for r in reserved:
+                self.cache.rollback(r)
+            for r in admitted:
+                self.cache.release(r)
+            raise
+        for t, row in zip(trees, result):
+            self.cache.commit(t.req_id, row[0])
+        self.steps_run += 1
+        self.tokens_run += M
+        return [row[1:1 + row[0]] for row in result]
 
     # ------------------------------------------------------------------ decode steps from CUDA graphs
     @staticmethod

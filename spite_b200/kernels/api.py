@@ -245,7 +245,8 @@ class KernelSet:
     def qk_prepare(self, qkv, q_out, batch, cache, *, num_heads, rotation, qk_norm, temperature,
                    value_mix=None, gates_out=None, bias=None, q_only=False, norm_dim=None, value_rotation=None,
                    values_are_keys=False):
-        """Encode positions of q and k, normalise, scale q, append k and v to the cache.
+        """Encode positions of q and k, normalise, scale q, append k and v to the cache (at the rows that `batch.slot_maps` names, if the
+        step has them, else at their positions).
         `bias` float32 [(nq + 2 nkv) hd]: added to the projection's columns before anything else.  `q_only`: a row of
         qkv holds the q heads alone (and `bias` theirs): the layer reads keys and values that another layer cached.
         qkv [M, >= (nq + 2 nkv) hd] T -> q_out [M, nq hd] T; `cache` is a `LayerCache`.

@@ -56,7 +56,8 @@ class QkPrepareParams(C.Structure):
                 ("v_mix_dim", C.c_int), ("v_mix", C.c_float), ("gates_out", C.c_void_p),
                 ("bias", C.c_void_p), ("q_only", C.c_int), ("norm_dim", C.c_int),
                 ("v_inv_freq", C.c_void_p), ("v_rotary_dim", C.c_int), ("v_pairing", C.c_int),
-                ("inv_freq_low", C.c_void_p), ("v_inv_freq_low", C.c_void_p), ("values_are_keys", C.c_int)]
+                ("inv_freq_low", C.c_void_p), ("v_inv_freq_low", C.c_void_p), ("values_are_keys", C.c_int),
+                ("slot_map", C.c_void_p)]
 
 
 class AttentionParams(C.Structure):
@@ -1054,6 +1055,12 @@ class CudaKernels(KernelSet):
                             v_mix=float(v_lam), gates_out=_ptr(gates_out), bias=_ptr(bias), q_only=int(bool(q_only)),
                             norm_dim=int(norm_dim or 0), v_inv_freq=v_freq, v_rotary_dim=v_dims, v_pairing=v_pairing,
                             inv_freq_low=low, v_inv_freq_low=v_low, values_are_keys=int(bool(values_are_keys)))
+        slot_maps = getattr(batch, "slot_maps", None)
+        if slot_maps is not None and cache.write:
+            slots = self._t(slot_maps[cache.group], torch.int64, "slot_map")
+            if slots.numel() < qkv.shape[0]:
+                raise KernelError(f"qk_prepare: the slot map has {slots.numel()} rows for {qkv.shape[0]} tokens")
+            p.slot_map = slots.data_ptr()
         b, c = self._step_tokens(batch, cache.group), self._paged(cache)
         st = self._lib("attention").spite_qk_prepare(self._dt, C.byref(p), C.byref(b), C.byref(c), self._stream())
         self._count("attention", 1)

@@ -70,6 +70,7 @@ class PagedAttention(Mixer):
         the row by the distance between query and key as `distance_rows` says."""
         super().__init__(ctx)
         self.conv_taps = None if conv_taps is None else int(conv_taps)
+        self.follows_trees = self.conv_taps in (None, 1)      # (a convolution over time knows one token before each)
         if self.conv_taps is not None and (self.conv_taps < 1 or self.conv_taps > 8):
             raise ConfigError(f"conv_taps {conv_taps} must lie in 1..8")
         if self.conv_taps is not None and kv_shared:
@@ -353,8 +354,12 @@ class PagedAttention(Mixer):
             more["score_softcap"] = self.score_softcap
         if self.distance_bias is not None:
             more["distance_bias"] = self.distance_bias
-        k.paged_attention(q, o, batch, cache, num_heads=self.nq, window=self.window,
-                          softmax_scale=self.softmax_scale, cache_settled=True, sink_logit=self.sink_logit, **more)
+        if getattr(batch, "ancestors", None) is None:
+            k.paged_attention(q, o, batch, cache, num_heads=self.nq, window=self.window,
+                              softmax_scale=self.softmax_scale, cache_settled=True, sink_logit=self.sink_logit, **more)
+        else:
+            k.tree_attention(q, o, batch, cache, num_heads=self.nq, window=self.window, softmax_scale=self.softmax_scale,
+                             sink_logit=self.sink_logit, **more)
         if self.output_gate:
             k.head_norm_gate(o, o, heads=self.nq, size=self.hd, gates=qkv, gate_column=self.head_columns)
         return o

@@ -181,6 +181,9 @@ class Mixer(Part):
     #: stream's shape that holds nothing yet) with its output instead of adding to it.  An arrangement that norms a
     #: sublayer's output before it joins the stream asks for this; for parts without it the arrangement zeroes the buffer.
     can_store = False
+    #: the part runs in a step that verifies drafted trees (`StepBatch.ancestors`): what it does to a token depends on the tokens that the token's
+    #: ancestor set names and on nothing that another token of the step leaves behind
+    follows_trees = False
     #: width of the concatenated heads in front of the output projection, for mixers whose forward is
     #: `heads` followed by one product with the parameter `o_proj` [hidden, heads_size]; None: not such a mixer
     heads_size = None

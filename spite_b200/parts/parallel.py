@@ -28,6 +28,7 @@ class ParallelMixers(Mixer):
         self.n_left, self.n = self.sides["left"].heads_size, sum(m.heads_size for m in self.sides.values())
         self.kernel_libraries = tuple(sorted({lib for m in self.sides.values() for lib in m.kernel_libraries}))
         self.graph_safe = all(m.graph_safe for m in self.sides.values())
+        self.follows_trees = all(m.follows_trees for m in self.sides.values())
         self.side_by_side = True              # the right mixer on a side stream
         self.wo = None
         self.cache_request()                  # (two mixers that want the same kind of cache are refused here)
