@@ -319,7 +319,8 @@ class KernelSet:
         of the way's nodes move to the places that follow the request's cached tokens: in every cache of `caches`, a list of (kv [caches, planes,
         pages, kv heads, page_size, head_dim], slot_map [M] int64, key_scales [caches, pages, kv heads, page_size] float32 or None), the row of
         slot_map[node] goes to slot_map[number on the way] (no row where either is negative).  With `lengths` (int32 [rows], and `lengths_out`, which may
-        be the same): lengths_out[slots[s]] = lengths[slots[s]] + counts[s] (without `slots`: row s)."""
+        be the same): lengths_out[slots[s]] = lengths[slots[s]] + counts[s] (without `slots`: row s).  Every row of `slots`, every row of a slot map and every
+        cache is named once."""
         raise NotImplementedError
 
     # ---- attention through latents

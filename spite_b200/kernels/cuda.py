@@ -148,6 +148,7 @@ class AttnDecodeExtra(C.Structure):
 
 # The arguments of the calls of a step of drafted tokens, packed as the C structures lie in memory.
 _TREE_CALL = struct.Struct("PPiiififPPPifPPi4x" "PPPii" "PqiiiiP" "PPii")         # AttentionParams, StepTokens, PagedCache, TreeStep
+_MOST = 0x7fffffff
 _LAYOUT_CALL = struct.Struct("15P11i4x")                                          # LayoutParams
 _ACCEPT_GROUPS = 8
 _ACCEPT_GROUP = struct.Struct("PPPq6i")                                           # AcceptGroup
@@ -1273,12 +1274,17 @@ class CudaKernels(KernelSet):
 
     def tree_attention(self, q, out, batch, cache, *, num_heads, window, softmax_scale, sink_logit=None, head_sinks=None, head_slopes=None,
                        head_gates=None, out_by_head=False, score_softcap=None, distance_bias=None):
-        what = "tree_attention"
-        self._check_attention(what, q, out, num_heads, softmax_scale, head_sinks, head_slopes, head_gates, score_softcap, distance_bias)
+        what, device = "tree_attention", torch.cuda.current_device()
+        for t in (q, out):
+            if t.dtype is not self.dtype or t.get_device() != device or not t.is_contiguous():
+                raise KernelError(f"{what}: q and out must be contiguous {self.dtype} tensors on the current device, cuda:{device}")
+        if out.numel() != q.numel() or not softmax_scale > 0:
+            raise KernelError(f"{what}: out must have as many elements as q, and the score scale be positive")
+        if not (head_sinks is head_slopes is head_gates is score_softcap is distance_bias is None):
+            self._check_attention(what, q, out, num_heads, softmax_scale, head_sinks, head_slopes, head_gates, score_softcap, distance_bias)
         M, table, cu, positions, seg, sets = batch.n_tokens, batch.block_tables[cache.group], batch.cu_seqlens, batch.positions, batch.seg_of_token, batch.ancestors
         if sets is None:
             raise KernelError(f"{what}: the step has no ancestor sets")
-        device = torch.cuda.current_device()
         self._whole_numbers(what, device, "positions, seg_of_token and cu_seqlens", (positions, seg, cu), 1)
         self._whole_numbers(what, device, "block_table and ancestors", (table, sets), 2)
         kv, scales = cache.kv, cache.key_scale
@@ -1289,18 +1295,16 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: positions, seg_of_token and ancestors of {M} tokens and block_table of {S} requests are needed")
         if scales is not None and tuple(self._t(scales, torch.float32, "key_scale").shape) != (n_pages, kv_heads, page):
             raise KernelError("a cache's key factors are [pages, kv heads, page_size]")
-        if q.shape[0] != M or q.numel() != M * num_heads * hd or num_heads % kv_heads:
+        if num_heads < 1 or q.shape[0] != M or q.numel() != M * num_heads * hd or num_heads % kv_heads:
             raise KernelError(f"{what}: q {tuple(q.shape)} does not hold {M} tokens of {num_heads} heads of {hd} ({kv_heads} kv heads)")
         if hd > 256:
             raise KernelError(f"{what}: heads of {hd} elements; up to 256 are supported")
         if not M:
             return
-        if q.get_device() != device:
-            raise KernelError(f"{what}: q is on {q.device}, the current device is cuda:{device}")
         stream = self._raw_stream()
         has_sink = sink_logit is not None or head_sinks is not None
         call = _TREE_CALL.pack(
-            q.data_ptr(), out.data_ptr(), num_heads, _WINDOW[window.kind], window.size, softmax_scale, has_sink, sink_logit or 0.0,
+            q.data_ptr(), out.data_ptr(), num_heads, _WINDOW[window.kind], min(window.size, _MOST), softmax_scale, has_sink, sink_logit or 0.0,
             _address(head_sinks), _address(head_slopes), _address(head_gates), M if out_by_head else 0, score_softcap or 0.0,
             0 if distance_bias is None else distance_bias.padded.data_ptr(), 0 if distance_bias is None else distance_bias.runs.data_ptr(),
             0 if distance_bias is None else distance_bias.length,
@@ -1361,7 +1365,7 @@ class CudaKernels(KernelSet):
             tables.data_ptr(), held.data_ptr(), _address(free), _address(n_free), slots.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), _address(parents),
             block.data_ptr(), cu.data_ptr(), positions.data_ptr(), seg.data_ptr(), slot_map.data_ptr(), _address(sets), status.data_ptr(),
             R, W, 0 if free is None else free.numel(), S, out_width, M, 0 if parents is None else parents.numel(), n_words, pages.page_size,
-            _WINDOW[pages.window.kind], pages.window.size)
+            _WINDOW[pages.window.kind], min(pages.window.size, _MOST))
         # one block while there is little to write, then a cluster of eight, then two launches (see `layout_words`)
         words = S * out_width + M * (4 + n_words)
         blocks = 0 if S > 512 or words > self.layout_words[1] else 1 if words <= self.layout_words[0] else 8

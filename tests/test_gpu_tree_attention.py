@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from draft_helpers import TreeCase, tolerance
-from spite_b200.cache import Window
+from spite_b200.cache import LayerCache, Window
 from spite_b200.kernels.api import DistanceBias, KernelError
 
 pytestmark = pytest.mark.gpu
@@ -191,6 +191,36 @@ def test_two_calls_at_once(kernels):
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
 
 
+@pytest.mark.parametrize("dtype,size", [(BF, 128), (F32, 128)])
+def test_beyond_32_bits(kernels, dtype, size):
+    """A cache of more than 2^31 elements whose pages in use lie at its far end."""
+    k = kernels[dtype]
+    case = TreeCase([200, 40], [20, 30], heads=4, kv_heads=1, size=size, dtype=dtype, seed=12)
+    want = run(kernels, case)
+    n, more = case.kv.shape[1], 150000
+    big = torch.zeros((2, more, 1, 64, size), dtype=dtype, device=DEV)                  # 1.2 * 10^9 elements a plane
+    big[:, more - n:] = case.kv.to(DEV)
+    q, batch, _ = case.step(DEV)
+    table = batch.block_tables[0]
+    batch.block_tables[0] = torch.where(table >= 0, table + (more - n), table)
+    out = torch.empty_like(q)
+    k.tree_attention(q, out, batch, LayerCache(0, big, None, 64, False), num_heads=4, window=FULL, softmax_scale=size ** -0.5)
+    assert torch.equal(out, want)
+
+
+def test_pages_that_are_not_there(kernels):
+    """A table's holes and page numbers outside the cache are not read: what they would hold is seen by nobody, or is another page's."""
+    for dtype, size in ((BF, 64), (F32, 64)):
+        case = TreeCase([70, 130], [5, 6], heads=2, kv_heads=1, size=size, dtype=dtype, seed=3)
+        q, batch, cache = case.step(DEV)
+        out = torch.zeros_like(q)
+        for bad in (-1, -(1 << 31), 1 << 30, case.kv.shape[1]):
+            batch.block_tables[0][:] = bad
+            kernels[dtype].tree_attention(q, out, batch, cache, num_heads=2, window=FULL, softmax_scale=0.125)
+        torch.cuda.synchronize()
+        assert not kernels[dtype].errors()
+
+
 def test_refusals(kernels):
     k = kernels[F32]
     case = TreeCase([9], [4], heads=4, kv_heads=2, size=16, seed=1)
@@ -198,7 +228,7 @@ def test_refusals(kernels):
     out = torch.empty_like(q)
     call = lambda **kw: k.tree_attention(kw.pop("q", q), kw.pop("out", out), batch, cache,
                                          **{**dict(num_heads=4, window=FULL, softmax_scale=0.25), **kw})
-    for kw in (dict(num_heads=3), dict(softmax_scale=0.0), dict(score_softcap=-1.0), dict(out=out[:2]), dict(q=q[:3], out=out[:3]), dict(q=q.bfloat16()),
+    for kw in (dict(num_heads=3), dict(num_heads=0), dict(softmax_scale=0.0), dict(score_softcap=-1.0), dict(out=out[:2]), dict(q=q[:3], out=out[:3]), dict(q=q.bfloat16()),
                dict(head_sinks=torch.zeros(3, device=DEV)), dict(q=q.t())):
         with pytest.raises(KernelError):
             call(**kw)
