@@ -215,7 +215,7 @@ class Engine:
         trees = [t if isinstance(t, DraftTree) else DraftTree(*t) for t in trees]
         self.check()
         if not all(part.follows_trees for _, part in self.model.parts() if isinstance(part, Mixer)):
-            raise StepError("drafted trees need layers without a state per request: one of the model's mixers keeps one")
+            raise StepError("drafted trees need attention over cached keys and values in every layer: one of the model's mixers is of another kind")
         vocab, seen = self.model.plan.vocab_size, set()
         for t in trees:
             n = len(t.tokens)

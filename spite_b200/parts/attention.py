@@ -70,7 +70,7 @@ class PagedAttention(Mixer):
         the row by the distance between query and key as `distance_rows` says."""
         super().__init__(ctx)
         self.conv_taps = None if conv_taps is None else int(conv_taps)
-        self.follows_trees = self.conv_taps in (None, 1)      # (a convolution over time knows one token before each)
+        self.follows_trees = self.conv_taps is None           # (a convolution over time knows one token before each)
         if self.conv_taps is not None and (self.conv_taps < 1 or self.conv_taps > 8):
             raise ConfigError(f"conv_taps {conv_taps} must lie in 1..8")
         if self.conv_taps is not None and kv_shared:

@@ -81,7 +81,7 @@ GROUP = dict(kv=SOME, scales=0, slot_map=SOME, plane_bytes=4096, planes=2, cache
     *[({n: 0}, {}, BAD) for n in ("tokens", "targets", "cu", "counts", "path", "emitted", "requests", "depth")],
     (dict(n=-1), {}, BAD), (dict(lengths=SOME, rows=1), {}, BAD), (dict(lengths=SOME, lengths_out=SOME), {}, BAD), (dict(n_groups=-1), {}, BAD),
     *[({}, {n: 0}, BAD) for n in ("kv", "slot_map", "planes", "caches", "pages", "heads", "page", "row")],
-    (dict(depth=1025), {}, UNSUPPORTED), (dict(n_groups=9), {}, UNSUPPORTED)])
+    (dict(depth=1025), {}, UNSUPPORTED), (dict(n_groups=9), {}, UNSUPPORTED), ({}, dict(row=255), UNSUPPORTED)])
 def test_accept_drafts(change, group, status):
     f = entry("drafts", "spite_accept_drafts", C.c_char_p, C.c_int, C.c_void_p)
     call = cuda._ACCEPT_CALL.pack(*{**ACCEPT, **change}.values(), cuda._ACCEPT_GROUP.pack(*{**GROUP, **group}.values()))
