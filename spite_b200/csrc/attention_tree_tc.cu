@@ -24,6 +24,16 @@
 // that is no node's (padding, what lies behind the last node) may hold anything, and 0 x NaN is NaN: the softmax warps clear
 // these rows of the tile in shared memory before the product.  Settled rows are finite as everywhere in the cache.
 //
+// Measured (40 query heads on 8 of 128 elements, device time with both kernels): one request of 131,072 keys, up to 25 nodes (singles) 97 to 103 us,
+// 5.2 to 5.6 TB/s: memory; 50 nodes (pairs) 162 us, 826 TFLOP/s, and 100 nodes 884: a pair's key tile takes 1.25 us, the chain scores -> softmax
+// -> product of a half, whose gaps the other half fills only in part (tensor pipe 43 % busy, special functions 42 %); heads of 64 elements have
+// the same chain for half the bytes, 0.75 us a key tile for a single (3.2 TB/s) and 1.3 for a pair.  8 requests of 16 nodes and 8,192 keys: 64 us,
+// 4.3 TB/s; one of 8 nodes and 100 keys: 7.5 us, half of it the start.  Measured and not kept: two threads a row (sixteen softmax warps; 405 against
+// 381 us for 16 requests of 64 nodes, 8,192 keys, 64 heads), part of the exponentials by a polynomial on the multiply-add units (390 against 355:
+// the loop outgrows the instruction cache), no turns at the exponentials or turns passed on after a half or seven eighths of a tile (within 3 %),
+// registers moved to the softmax warps (no change), a half's state handed over before its last product (168 against 163), other costs of a tile
+// and an item within a factor of 1.5 (within 5 %).
+//
 // Score, mask and softmax: crates/spite-compute/src/flash_attn.rs:111-156, with the mask of attention_tree.cuh.  Every wait is bounded
 // (see tcgen05.cuh); codes: 1 a loader, 2 tensor-core issue, 3 softmax.
 #include "attention_tree.cuh"
@@ -640,7 +650,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
 // Adds up the parts of the items that were cut, in the order of the keys.  grid (blocks, head_dim / JOIN_COLS, row tiles of a pair), a thread a row;
 // part 0 of an item is the last of the block before its first cut, part k the first of the block behind its cut k.  What it costs is the latency of
-// its loads, so as many as there are registers for are asked for at once.
+// its loads, so as many as there are registers for are asked for at once.  (As many blocks as fit beside each other, with a list of the items that
+// were cut, were no faster: 8 x 16 nodes, 8,192 keys 63.7 against 62.9 to 67.6 us in all, 16 nodes and 1,000 keys 20 against 17, 16 x 64 nodes 333 against 341.)
 constexpr int JOIN_COLS = 8;
 __global__ void __launch_bounds__(BM) attn_tree_tc_join_kernel(const AttentionParams p, const TreeCut cut, int nkv, int tpt, int hd) {
     pdl_wait();

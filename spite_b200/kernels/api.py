@@ -309,7 +309,9 @@ class KernelSet:
         whose parent is not smaller has none.  With `parents` or `ancestors` a request brings up to 1024 tokens.
         What only the device can see is said in out.status: `StepLayout.OUT_OF_PAGES`, or MALFORMED (a slot twice or outside the tables, a
         length that the row does not cover, more tokens or pages than `out` has room for); then nothing of `pages` has changed, block_table is -1
-        and the step has no tokens.  `lengths` stays as it is.  Calling it again with the same lengths takes no further pages."""
+        and the step has no tokens.  `lengths` stays as it is.  Calling it again with the same lengths takes no further pages.  A page that comes
+        off the stack holds what it held before: `tree_attention` reads only what is some token's, `paged_attention` wants finite numbers in the rest of
+        it (a pool that was zeroed once has them)."""
         raise NotImplementedError
 
     def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
