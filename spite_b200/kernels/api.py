@@ -294,7 +294,7 @@ class KernelSet:
         it, and its row of the cache may hold anything, as may the rows behind the last node), unless its window ends behind
         their position.  Distances are between positions.  A row that sees nothing is zero.  Everything else as in `paged_attention`;
         `batch` needs positions, seg_of_token, cu_seqlens, block_tables and ancestors, and the host need not know how much is cached.  Rows of
-        `out` behind the last request's are left as they were."""
+        `out` behind the last request's are left as they were.  `out` shares no memory with `q`."""
         raise NotImplementedError
 
     # ---- steps laid out and drafts accepted on the device
@@ -322,7 +322,7 @@ class KernelSet:
         pages, kv heads, page_size, head_dim], slot_map [M] int64, key_scales [caches, pages, kv heads, page_size] float32 or None), the row of
         slot_map[node] goes to slot_map[number on the way] (no row where either is negative).  With `lengths` (int32 [rows], and `lengths_out`, which may
         be the same): lengths_out[slots[s]] = lengths[slots[s]] + counts[s] (without `slots`: row s).  Every row of `slots`, every row of a slot map and every
-        cache is named once."""
+        cache is named once; counts, path and emitted share no memory with the rest."""
         raise NotImplementedError
 
     # ---- attention through latents
