@@ -148,7 +148,13 @@ class AttnDecodeExtra(C.Structure):
 
 # The arguments of the calls of a step of drafted tokens, packed as the C structures lie in memory.
 _TREE_CALL = struct.Struct("PPiiififPPPifPPi4x" "PPPii" "PqiiiiP" "PPii")         # AttentionParams, StepTokens, PagedCache, TreeStep
-_MOST = 0x7fffffff
+_MOST = 0x7fffffff           # of a window's size
+_DRAFT_ENTRIES = {            # what the entries that take packed arguments are called with
+    "spite_tree_attention": (C.c_int, C.c_char_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p),
+    "spite_tree_attention_tc": (C.c_char_p, C.c_int, C.c_void_p, C.c_longlong, C.c_void_p),
+    "spite_layout_step": (C.c_char_p, C.c_int, C.c_void_p),
+    "spite_accept_drafts": (C.c_char_p, C.c_int, C.c_void_p),
+}
 _LAYOUT_CALL = struct.Struct("15P11i4x")                                          # LayoutParams
 _ACCEPT_GROUPS = 8
 _ACCEPT_GROUP = struct.Struct("PPPq6i")                                           # AcceptGroup
@@ -460,11 +466,11 @@ class CudaKernels(KernelSet):
         return out
 
     @staticmethod
-    def _raw_stream() -> int:
+    def _raw_stream(device=None) -> int:
         # The handle by a name that torch's own compiler uses but does not document: a Stream object for each of a step's launches takes
         # about 1.5 us more.  A torch without the name gets the object.
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
+        return raw(torch.cuda.current_device() if device is None else device) if raw else torch.cuda.current_stream().cuda_stream
 
     @staticmethod
     def _stream():
@@ -1257,11 +1263,11 @@ class CudaKernels(KernelSet):
 
     # The calls of a step of drafted tokens stand between its other launches, where the host's time counts as much as the kernels': their
     # arguments are packed in one go (0.3 us; a ctypes structure by field names 1.7) and go through entries with declared types.
-    def _entry(self, library, name, *argtypes):
+    def _entry(self, library, name):
         f = self._entries.get(name)
         if f is None:
             f = self._entries[name] = getattr(self._lib(library), name)
-            f.argtypes = argtypes
+            f.argtypes = _DRAFT_ENTRIES[name]
         return f
 
     @staticmethod
@@ -1301,7 +1307,7 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: heads of {hd} elements; up to 256 are supported")
         if not M:
             return
-        stream = self._raw_stream()
+        stream = self._raw_stream(device)
         has_sink = sink_logit is not None or head_sinks is not None
         call = _TREE_CALL.pack(
             q.data_ptr(), out.data_ptr(), num_heads, _WINDOW[window.kind], min(window.size, _MOST), softmax_scale, has_sink, sink_logit or 0.0,
@@ -1315,7 +1321,7 @@ class CudaKernels(KernelSet):
                 and self.use_tcgen05_attention:
             n_floats = self.sm_count * (4 * (hd + 2) * 128 + 4)
             part = torch.empty(n_floats, dtype=torch.float32, device=q.device)
-            st = self._entry("attention_tree_tc", "spite_tree_attention_tc", C.c_char_p, C.c_int, C.c_void_p, C.c_longlong, C.c_void_p)(
+            st = self._entry("attention_tree_tc", "spite_tree_attention_tc")(
                 call, self.sm_count, part.data_ptr(), n_floats, stream)
             if st != -2:                        # -2: more than 128 heads a kv head, a tensor that does not start at 16 bytes, sizes beyond 32 bits
                 self._count("attention_tree_tc", 2)
@@ -1331,7 +1337,7 @@ class CudaKernels(KernelSet):
         splits = max(1, min(32, 8 * self.sm_count // blocks, -(-keys // 128)))
         share = -(-keys // splits)
         part = torch.empty(M * num_heads * splits * (-(-hd // 4) * 4 + 4), dtype=torch.float32, device=q.device) if splits > 1 else None
-        st = self._entry("attention_tree", "spite_tree_attention", C.c_int, C.c_char_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p)(
+        st = self._entry("attention_tree", "spite_tree_attention")(
             self._dt, call, _address(part), 0 if part is None else part.numel(), splits, share, stream)
         self._count("attention_tree", 1 + (splits > 1))
         _check(st, what)
@@ -1369,7 +1375,7 @@ class CudaKernels(KernelSet):
         # one block while there is little to write, then a cluster of eight, then two launches (see `layout_words`)
         words = S * out_width + M * (4 + n_words)
         blocks = 0 if S > 512 or words > self.layout_words[1] else 1 if words <= self.layout_words[0] else 8
-        st = self._entry("drafts", "spite_layout_step", C.c_char_p, C.c_int, C.c_void_p)(call, blocks, self._raw_stream())
+        st = self._entry("drafts", "spite_layout_step")(call, blocks, self._raw_stream(device))
         self._count("drafts", 1 if blocks else 2)
         _check(st, what)
 
@@ -1398,7 +1404,7 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: {len(caches)} groups of caches; up to {_ACCEPT_GROUPS} in one call")
         groups, most = [], 1
         for kv, slot_map, scales in caches:
-            if self._t(kv, self.dtype, f"{what}: cache").dim() != 6 or not kv.numel():
+            if self._t(kv, self.dtype, "accept_drafts: cache").dim() != 6 or not kv.numel():
                 raise KernelError(f"{what}: a cache is [caches, planes, pages, kv heads, page_size, head_dim]")
             self._whole_numbers(what, device, "slot_map", (slot_map,), 1, torch.int64)
             if slot_map.numel() < M:
@@ -1415,7 +1421,7 @@ class CudaKernels(KernelSet):
                                  b"".join(groups))
         # a thread for every 16 bytes of a token's rows, as long as that is not far more blocks than the device holds
         pieces = max(1, min(-(-most // 256), max(1, 16 * self.sm_count // S)))
-        st = self._entry("drafts", "spite_accept_drafts", C.c_char_p, C.c_int, C.c_void_p)(call, pieces, self._raw_stream())
+        st = self._entry("drafts", "spite_accept_drafts")(call, pieces, self._raw_stream(device))
         self._count("drafts", 1)
         _check(st, what)
 
