@@ -1350,13 +1350,9 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: a stack of free pages needs its height, and the other way round")
         device = torch.cuda.current_device()
         self._whole_numbers(what, device, "tables, block_table and ancestors", (tables, block) if sets is None else (tables, block, sets), 2)
-        self._whole_numbers(what, device, "held, slots, lengths, new_tokens, cu_seqlens, positions, seg_of_token and status",
-                            (held, slots, lengths, new_tokens, cu, positions, seg, status), 1)
+        self._whole_numbers(what, device, "held, slots, lengths, new_tokens, cu_seqlens, positions, seg_of_token, status, free_pages, n_free and parents",
+                            [t for t in (held, slots, lengths, new_tokens, cu, positions, seg, status, free, n_free, parents) if t is not None], 1)
         self._whole_numbers(what, device, "slot_map", (slot_map,), 1, torch.int64)
-        if free is not None:
-            self._whole_numbers(what, device, "free_pages and n_free", (free, n_free), 1)
-        if parents is not None:
-            self._whole_numbers(what, device, "parents", (parents,), 1)
         S, (R, W), M, (block_rows, out_width) = slots.numel(), tables.shape, positions.numel(), block.shape
         n_sets, n_words = (M, 0) if sets is None else sets.shape
         if held.numel() != R or lengths.numel() != R or new_tokens.numel() != S or block_rows != S or cu.numel() != S + 1:
@@ -1381,11 +1377,9 @@ class CudaKernels(KernelSet):
 
     def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
         what, device = "accept_drafts", torch.cuda.current_device()
-        self._whole_numbers(what, device, "tokens, targets, cu_seqlens and counts", (tokens, targets, cu_seqlens, counts), 1)
+        self._whole_numbers(what, device, "tokens, targets, cu_seqlens, counts, parents, slots, lengths and lengths_out",
+                            [t for t in (tokens, targets, cu_seqlens, counts, parents, slots, lengths, lengths_out) if t is not None], 1)
         self._whole_numbers(what, device, "path and emitted", (path, emitted), 2)
-        for name, t in (("parents", parents), ("slots", slots), ("lengths", lengths), ("lengths_out", lengths_out)):
-            if t is not None:
-                self._whole_numbers(what, device, name, (t,), 1)
         S, M, (rows, depth) = cu_seqlens.numel() - 1, tokens.numel(), path.shape
         if targets.numel() != M or (parents is not None and parents.numel() != M):
             raise KernelError(f"{what}: {M} tokens have a parent and a target each")
@@ -1404,12 +1398,13 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: {len(caches)} groups of caches; up to {_ACCEPT_GROUPS} in one call")
         groups, most = [], 1
         for kv, slot_map, scales in caches:
-            if self._t(kv, self.dtype, "accept_drafts: cache").dim() != 6 or not kv.numel():
+            shape = self._t(kv, self.dtype, "accept_drafts: cache").shape
+            if len(shape) != 6 or 0 in shape:
                 raise KernelError(f"{what}: a cache is [caches, planes, pages, kv heads, page_size, head_dim]")
             self._whole_numbers(what, device, "slot_map", (slot_map,), 1, torch.int64)
             if slot_map.numel() < M:
                 raise KernelError(f"{what}: the slot map has {slot_map.numel()} rows for {M} tokens")
-            n, planes, n_pages, heads, page, size = kv.shape
+            n, planes, n_pages, heads, page, size = shape
             if scales is not None and tuple(self._t(scales, torch.float32, f"{what}: key_scales").shape) != (n, n_pages, heads, page):
                 raise KernelError(f"{what}: key_scales are [caches, pages, kv heads, page_size]")
             row_bytes = size * kv.element_size()
