@@ -41,7 +41,7 @@ namespace {
 constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32;
 constexpr int FEW_PAGES = 4;             // that a request's own thread takes
 
-__device__ __forceinline__ int first_needed(const LayoutParams& p, int len) {       // (a later token reads nothing before it)
+__host__ __device__ __forceinline__ int first_needed(const LayoutParams& p, int len) {       // (a later token reads nothing before it)
     if (p.window_kind == 1) return len / p.window_size * p.window_size;
     if (p.window_kind == 2) return max(0, len - p.window_size + 1);
     return 0;
@@ -83,10 +83,13 @@ struct Known { int cu[PLAN_THREADS + 1], row[PLAN_THREADS], len[PLAN_THREADS]; }
 
 struct Request { int row, fresh, len, held, need, goes_to, goes, at; };   // (goes: pages [goes_to - goes, goes_to) go back)
 
-// What request s of the step has and wants; a row of -1 where there is nothing to do, `ok` false where it cannot be right.
-__device__ __forceinline__ Request request_of(const LayoutParams& p, int s, bool& ok) {
+__host__ __device__ constexpr Request nothing() { return Request{-1, 0, 0, 0, 0, 0, 0, 0}; }
+
+// What request s of the step has and wants; nothing where there is nothing to do, or where it cannot be right (`ok` false: none of its numbers
+// may index the tables then).
+__host__ __device__ __forceinline__ Request request_of(const LayoutParams& p, int s, bool& ok) {
     const int row = p.slots[s], fresh = p.new_tokens[s];
-    Request r{-1, 0, 0, 0, 0, 0, 0, 0};
+    Request r = nothing();
     ok = row >= -1 && row < p.n_rows && fresh >= -1;
     if (!ok || row < 0) return r;
     r = Request{row, fresh, p.lengths[row], p.held[row], 0, 0, 0, 0};
@@ -98,11 +101,11 @@ __device__ __forceinline__ Request request_of(const LayoutParams& p, int s, bool
         const unsigned end = (unsigned)r.len + (unsigned)fresh, pages = end / p.page_size + (end % p.page_size != 0);       // (len and fresh are below 2^31)
         ok = ok && r.len >= 0 && (long long)r.held * p.page_size >= r.len && end <= 0x7fffffffu && pages <= (unsigned)min(p.table_width, p.out_width) &&
              (p.free_pages || pages <= (unsigned)r.held) && fresh <= p.n_tokens && (!p.parents || fresh <= SPITE_MAX_DRAFTS) && (!p.ancestors || fresh <= 32 * p.n_words);
-        r.need = ok ? max(r.held, (int)pages) : r.held;
-        r.goes_to = ok && p.free_pages ? min(first_needed(p, r.len) / p.page_size, r.held) : 0;
+        if (!ok) return nothing();
+        r.need = max(r.held, (int)pages);
+        r.goes_to = p.free_pages ? min(first_needed(p, r.len) / p.page_size, r.held) : 0;
     }
-    if (!ok) r.row = -1;
-    return r;
+    return ok ? r : nothing();
 }
 
 // One block plans the step and changes the persistent state: whose pages go back, who gets which.  A thread a request, a warp a
@@ -122,12 +125,12 @@ __device__ void plan_step(const LayoutParams& p, Known* known) {
     // front of them a row holds -1.  A warp looks at them from above, 32 at a time.
     auto take_up = [&](int s0, bool check) {
         const int s = s0 + threadIdx.x;
-        Request r{-1, 0, 0, 0, 0, 0, 0, 0};
+        Request r = nothing();
         if (s < p.n_requests) {
             bool ok;
             r = request_of(p, s, ok);
             if (check && ok && r.row >= 0) ok = (atomicOr(&seen[r.row / 32], 1u << (r.row % 32)) >> (r.row % 32) & 1u) == 0;
-            if (!ok) { bad = SPITE_LAYOUT_MALFORMED; r.row = -1; }
+            if (!ok) { bad = SPITE_LAYOUT_MALFORMED; r = nothing(); }
         }
         if (r.goes_to > 0 && p.tables[(size_t)r.row * p.table_width + r.goes_to - 1] < 0) r.goes_to = 0;     // (they have gone already)
         reqs[threadIdx.x] = r;
@@ -152,7 +155,7 @@ __device__ void plan_step(const LayoutParams& p, Known* known) {
     const int n_free = p.free_pages ? *p.n_free : 0;
     long long total[3] = {0, 0, 0}, before[3];                 // tokens, pages back, pages taken
     const bool one = p.n_requests <= PLAN_THREADS;             // (what is known of the requests then stays in place)
-    Request r{-1, 0, 0, 0, 0, 0, 0, 0};
+    Request r = nothing();
     for (int s0 = 0; s0 < p.n_requests; s0 += PLAN_THREADS) {
         r = take_up(s0, true);
         int v[3] = {max(r.fresh, 0), r.goes, r.fresh >= 0 ? r.need - r.held : 0};
@@ -214,7 +217,7 @@ __device__ void plan_step(const LayoutParams& p, Known* known) {
         if (!one) {
             bool ok;
             const int s = s0 + threadIdx.x;
-            r = Request{-1, 0, 0, 0, 0, 0, 0, 0};
+            r = nothing();
             if (s < p.n_requests) r = request_of(p, s, ok);
             int v[3] = {0, 0, r.fresh >= 0 ? r.need - r.held : 0};
             scan3(v, scratch, taken, before);
