@@ -13,6 +13,10 @@
 // as a running maximum and sum; shares of the keys leave their unnormalised results, which a second kernel adds up in the order of the keys.  The rows
 // of the cache that are no visible token's are read as zeros, so they may hold anything.
 //
+// NaN, infinities and numbers next to the largest cannot be split; and the products would carry a value that is not finite into rows that do not see
+// it, 0 x NaN being NaN.  Where a tile has such a number, the warps that meet it make their products again one by one in float32, with a row's own
+// keys alone.  Looking for them takes 1 to 3 % (8 requests of 16 nodes, 2,048 keys, 40 heads on 8 of 128: 271 us, 265 without).
+//
 // Score, mask and softmax: crates/spite-compute/src/flash_attn.rs:111-156, with the mask of attention_tree.cuh.
 #include "attention_tree.cuh"
 
@@ -23,18 +27,41 @@ constexpr int THREADS = 256;
 constexpr int JOIN_THREADS = 128;
 constexpr int P_STRIDE = ROWS + 8;       // of a key's weights: four keys x eight rows lie in different banks
 
-// A number as the products take it: rounded to 11 bits, and what that leaves, rounded to 11 bits (the products take the upper bits).
+// A number as the products take it: rounded to 11 bits, and what that leaves, rounded to 11 bits (the products take the upper bits).  NaN, infinity
+// and what rounds up to infinity do not come through that: they make `odd` NaN, which stays zero otherwise.
 struct Split { unsigned hi, lo; };
 __device__ __forceinline__ Split split(float v) {
     const unsigned hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
     return Split{hi, __float_as_uint(v - __uint_as_float(hi)) + 0x1000u};
 }
+__device__ __forceinline__ Split split(float v, float& odd) {
+    const Split s = split(v);
+    odd = fmaf(v - __uint_as_float(s.hi), 0.f, odd);
+    return s;
+}
+__device__ __forceinline__ bool splits(float v) { return fabsf(v) < 0x1.ffep127f; }
+// A stored bfloat16 is its own upper bits, and comes through the products whatever it is.
+__device__ __forceinline__ Split split(__nv_bfloat16 v, float&) { return Split{__float_as_uint(to_f32(v)), 0u}; }
 // d += a b for 16 x 8 and 8 x 8 numbers; lane 4 g + c holds a's rows g, g + 8 of columns c, then of c + 4; b's column g of rows c, c + 4;
 // d's rows g (two columns from 2 c on) and g + 8.
 __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// What a row weighs a key with that it does not see: zero, and by its sign apart from a weight that has become zero.
+constexpr float UNSEEN = -0.f;
+// A query's product with a key, and a row's sum over a column of the values that it sees (`weights` P_STRIDE apart, `column` `stride`), in float32.
+template <typename T> __device__ __noinline__ float product(const float* q, const T* k, int n) {
+    float sum = 0.f;
+    for (int d = 0; d < n; ++d) sum = fmaf(q[d], to_f32(k[d]), sum);
+    return sum;
+}
+template <typename T> __device__ __noinline__ float seen_values(const float* weights, const T* column, int stride, int n) {
+    float sum = 0.f;
+    for (int j = 0; j < n; ++j)
+        if (__float_as_uint(weights[j * P_STRIDE]) != __float_as_uint(UNSEEN)) sum = fmaf(weights[j * P_STRIDE], to_f32(column[j * stride]), sum);
+    return sum;
 }
 // 16 bytes from global to shared memory, or zeros.
 __device__ __forceinline__ void copy16(void* to, const void* from, bool there) {
@@ -164,13 +191,18 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
     const T* keys = (const T*)c.kv;
     const T* values = keys + c.v_offset;
     if (tile0 < tile1 && threadIdx.x < BN) note(find(tile0), 0);
+    bool q_odd = false;                                        // some number of q cannot be split
 #pragma unroll
     for (int i = 0; i < ROWS / 8; ++i) {
         const int r = warp + 8 * i;
         const T* q = (const T*)p.q + ((size_t)(t0 + (r < n_rows ? r / heads : 0)) * nq + kvh * G + h0 + (r < n_rows ? r % heads : 0)) * hd;
-        for (int d = lane; d < hd8; d += 32) q_s[r * q_stride + d] = r < n_rows && d < hd ? to_f32(q[d]) : 0.f;
+        for (int d = lane; d < hd8; d += 32) {
+            const float v = r < n_rows && d < hd ? to_f32(q[d]) : 0.f;
+            q_s[r * q_stride + d] = v;
+            q_odd |= !splits(v);
+        }
     }
-    __syncthreads();
+    q_odd = __syncthreads_or(q_odd);
     if (tile0 < tile1) fetch(k_s, k_stride, keys, 0);
 
     // Warps 2 (halves of the rows) x 4 (quarters of the tile's keys, then of the head); a thread's rows are g and g + 8 of the half.
@@ -206,6 +238,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
         __syncthreads();                                       // the keys are here
         float s[KT][4];                                        // [eight of keys][row g: two keys, row g + 8: two keys]
         unsigned vis = 0;                                      // bit 4 k + e: s[k][e] is a visible key's
+        float odd = 0.f;
         if (works) {
 #pragma unroll
             for (int k = 0; k < KT; ++k) s[k][0] = s[k][1] = s[k][2] = s[k][3] = 0.f;
@@ -228,7 +261,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                     }
 #pragma unroll
                     for (int k = 0; k < KT; ++k) {
-                        const Split u = split(to_f32(kr[8 * k * k_stride + d])), w = split(to_f32(kr[8 * k * k_stride + d + 4]));
+                        const Split u = split(kr[8 * k * k_stride + d], odd), w = split(kr[8 * k * k_stride + d + 4], odd);
                         const unsigned b_hi[2] = {u.hi, w.hi}, b_rest[2] = {u.lo, w.lo};
                         if (REST) {
                             mma(part[k], rest, b_hi);
@@ -241,6 +274,19 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                 for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[k][e] += part[k][e];
+            }
+            if (!REST) {                                       // (what bfloat16 keys and queries make that is not finite)
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd = fmaf(s[k][e], 0.f, odd);
+            }
+            if (__any_sync(0xffffffffu, odd != 0.f) || q_odd) {        // numbers that cannot be split: as the formula has it
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[k][e] = product(q_s + (16 * half + g + 8 * (e >> 1)) * q_stride, k_s + (quarter * 8 * KT + 8 * k + 2 * cc + (e & 1)) * k_stride, hd);
             }
             const int j0 = lo_any + ti * BN;
             if (plain && j0 >= lo_all && j0 + BN <= len) {     // settled keys that every row sees
@@ -287,13 +333,14 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                 const int r = 16 * half + g + 8 * i;
                 const float m_new = fmaxf(fmaxf(m[i], fmaxf(top_s[0][r], top_s[1][r])), fmaxf(top_s[2][r], top_s[3][r]));
                 if (m_new != -INFINITY) shrink[i] = expf(m[i] - m_new);
+                const float from = m_new == -INFINITY ? 0.f : m_new;           // (scores of minus infinity weigh nothing)
                 m[i] = m_new;
                 l[i] *= shrink[i];
 #pragma unroll
                 for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float w = vis >> (4 * k + 2 * i + e) & 1u ? expf(s[k][2 * i + e] - m_new) : 0.f;
+                        const float w = vis >> (4 * k + 2 * i + e) & 1u ? expf(s[k][2 * i + e] - from) : UNSEEN;
                         l[i] += w;                             // (of this thread's keys; the sums meet in the end)
                         p_s[(quarter * 8 * KT + 8 * k + 2 * cc + e) * P_STRIDE + r] = w;
                     }
@@ -304,6 +351,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
         if (works) {
 #pragma unroll
             for (int e = 0; e < 4 * HD4; ++e) { acc[e][0] *= shrink[0]; acc[e][1] *= shrink[0]; acc[e][2] *= shrink[1]; acc[e][3] *= shrink[1]; }
+            odd = 0.f;
             float part[4 * HD4][4];
 #pragma unroll
             for (int e = 0; e < 4 * HD4; ++e) part[e][0] = part[e][1] = part[e][2] = part[e][3] = 0.f;
@@ -314,18 +362,33 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                 unsigned hi[4], rest[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const Split v = split(wr[(j + (e >> 1) * 4) * P_STRIDE + (e & 1) * 8]);
+                    const Split v = split(wr[(j + (e >> 1) * 4) * P_STRIDE + (e & 1) * 8], odd);
                     hi[e] = v.hi;
                     rest[e] = v.lo;
                 }
 #pragma unroll
                 for (int e = 0; e < 4 * HD4; ++e) {
                     if (quarter * 32 * HD4 + 8 * e >= hd8) continue;                   // (the head ends before; the same for the warp)
-                    const Split u = split(to_f32(vr[j * v_stride + 8 * e])), w = split(to_f32(vr[(j + 4) * v_stride + 8 * e]));
+                    const Split u = split(vr[j * v_stride + 8 * e], odd), w = split(vr[(j + 4) * v_stride + 8 * e], odd);
                     const unsigned b_hi[2] = {u.hi, w.hi}, b_rest[2] = {u.lo, w.lo};
                     mma(part[e], rest, b_hi);
                     if (REST) mma(part[e], hi, b_rest);
                     mma(part[e], hi, b_hi);
+                }
+            }
+            if (!REST) {
+#pragma unroll
+                for (int e = 0; e < 4 * HD4; ++e)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) odd = fmaf(part[e][k], 0.f, odd);
+            }
+            if (__any_sync(0xffffffffu, odd != 0.f)) {
+#pragma unroll
+                for (int e = 0; e < 4 * HD4; ++e) {
+                    if (quarter * 32 * HD4 + 8 * e >= hd8) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        part[e][k] = seen_values(p_s + 16 * half + g + 8 * (k >> 1), v_s + quarter * 32 * HD4 + 8 * e + 2 * cc + (k & 1), v_stride, BN);
                 }
             }
 #pragma unroll
@@ -353,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
         float row_m = m[i], row_l = (l_s[0][r] + l_s[1][r]) + (l_s[2][r] + l_s[3][r]), scale = 1.f;
         if (n_splits == 1) {
             const float fold = tree_fold_sink(p, h, row_m, row_l);
-            scale = fold * gate_of(p, t, h) / fmaxf(row_l, 1e-30f);
+            scale = fold * gate_of(p, t, h) / tree_divisor(row_l);
         }
         T* out = (T*)p.out + out_row_of(p, t, h) * hd;
         float* part = partial + (((size_t)t * nq + h) * n_splits + split_no) * part_floats(hd);
@@ -366,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                 if (n_splits == 1) out[d + k] = from_f32<T>(acc[e][2 * i + k] * scale); else __stcg(part + d + k, acc[e][2 * i + k]);
             }
         }
-        if (n_splits > 1 && quarter == 0 && cc == 0) __stcg((float2*)(part + hdp), make_float2(row_m, row_l));
+        if (n_splits > 1 && quarter == 0 && cc == 0) __stcg((float2*)(part + hdp), tree_state(row_m, row_l));
     }
 }
 
@@ -401,7 +464,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_tree_join_kernel(const Atte
     const float my_w = ml.x == -INFINITY ? 0.f : expf(ml.x - m);
     float l = warp_sum(ml.y * my_w);
     const float shrink = tree_fold_sink(p, head, m, l);
-    const float scale = shrink * gate_of(p, t, head) / fmaxf(l, 1e-30f);
+    const float scale = shrink * gate_of(p, t, head) / tree_divisor(l);
     for (int s0 = 0; s0 < n_splits; s0 += N) {
         if (s0) ask(s0);
 #pragma unroll

@@ -34,6 +34,12 @@ __device__ __forceinline__ bool tree_node_is_real(const TreeStep& x, int first, 
     return i < 32 * x.n_words && (x.ancestors[(size_t)(first + i) * x.n_words + i / 32] >> (i % 32) & 1u);
 }
 
+// A row's maximum and sum as others read them: a sum that is NaN makes the maximum NaN (a row whose scores are all NaN has the maximum of a row
+// that sees nothing, minus infinity, and would be passed over).
+__device__ __forceinline__ float2 tree_state(float m, float l) { return make_float2(l != l ? l : m, l); }
+// What a row's values are divided by: its sum, NaN included, or for a row that sees nothing a number that leaves its zeros.
+__device__ __forceinline__ float tree_divisor(float l) { return l < 1e-30f ? 1e-30f : l; }
+
 // The sink folded into a row's finished state (as fold_sink); one of minus infinity adds nothing, also to a row that sees no key.
 __device__ __forceinline__ float tree_fold_sink(const AttentionParams& p, int head, float m, float& l) {
     return p.has_sink && sink_of(p, head) > -INFINITY ? fold_sink(p, head, m, l) : 1.f;

@@ -292,7 +292,8 @@ class KernelSet:
         (`batch.positions`) is len + its depth; node 0 has depth 0.  Node i sees the places below len that `window` lets its position see, and of
         the nodes up to itself those whose bit is set in its row and in their own (a node without its own bit is padding: nobody sees
         it, and its row of the cache may hold anything, as may the rows behind the last node), unless its window ends behind
-        their position.  Distances are between positions.  A row that sees nothing is zero.  Everything else as in `paged_attention`;
+        their position.  Distances are between positions.  A row that sees nothing, or scores of minus infinity alone, is zero; a NaN among what a row
+        sees makes the elements NaN that it goes into.  Everything else as in `paged_attention`;
         `batch` needs positions, seg_of_token, cu_seqlens, block_tables and ancestors, and the host need not know how much is cached.  Rows of
         `out` behind the last request's are left as they were.  `out` shares no memory with `q`."""
         raise NotImplementedError
