@@ -22,7 +22,8 @@
 //
 // Masks matter in the tiles at a window's end and in those with the step's own nodes; there a row makes 64 bits of what it sees.  A value row
 // that is no node's (padding, what lies behind the last node) may hold anything, and 0 x NaN is NaN: the softmax warps clear
-// these rows of the tile in shared memory before the product.  Settled rows are finite as everywhere in the cache.
+// these rows of the tile in shared memory before the product.  Settled rows are finite as everywhere in the cache; a value of a node or of a settled
+// row that is not reaches the other rows of its request, and a row whose sum is NaN is NaN.
 //
 // Measured (40 query heads on 8 of 128 elements, device time with both kernels): one request of 131,072 keys, up to 25 nodes (singles) 97 to 103 us,
 // 5.2 to 5.6 TB/s: memory; 50 nodes (pairs) 162 us, 826 TFLOP/s, and 100 nodes 884: a pair's key tile takes 1.25 us, the chain scores -> softmax
@@ -106,7 +107,7 @@ __device__ __forceinline__ float row_scale_of(const AttentionParams& p, int tok,
         shrink = m == -INFINITY ? 0.f : exp2f(m - m2);
         l = l * shrink + exp2f(sink2 - m2);
     }
-    return shrink * gate_of(p, tok, head) / fmaxf(l, 1e-30f);
+    return shrink * gate_of(p, tok, head) / tree_divisor(l);
 }
 
 // The n lowest of 64 bits.
@@ -601,12 +602,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         ld32(o, lane_base + 2 * BN + c0);
                         leave(o, c0, inv);
                     }
-                    if (part) __stcg((float2*)(slot + 2 * HD * BM) + g * BM + r, make_float2(m_ref, l));
+                    if (part) __stcg((float2*)(slot + 2 * HD * BM) + g * BM + r, tree_state(m_ref, l));
                 }
                 turns += n;
             } else {
                 // the halves' states and outputs are added up: each half takes half of the head, and reads the other's out of tensor memory
-                state_s[g][r] = make_float2(m_ref, l);
+                state_s[g][r] = tree_state(m_ref, l);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars.state_ready));
@@ -628,7 +629,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             o[e] = (fa != 0.f ? o[e] * fa : 0.f) + (fd != 0.f ? o1[e] * fd : 0.f);
                         leave(o, c0, inv);
                     }
-                    if (part && g == 0) __stcg((float2*)(slot + 2 * HD * BM) + r, make_float2(m, sum));
+                    if (part && g == 0) __stcg((float2*)(slot + 2 * HD * BM) + r, tree_state(m, sum));
                 }
                 fence_before();
                 __syncwarp();

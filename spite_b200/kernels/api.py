@@ -293,7 +293,7 @@ class KernelSet:
         the nodes up to itself those whose bit is set in its row and in their own (a node without its own bit is padding: nobody sees
         it, and its row of the cache may hold anything, as may the rows behind the last node), unless its window ends behind
         their position.  Distances are between positions.  A row that sees nothing, or scores of minus infinity alone, is zero; a NaN among what a row
-        sees makes the elements NaN that it goes into.  Everything else as in `paged_attention`;
+        sees makes the elements NaN that it goes into (bfloat16: values that are not finite may reach rows of the request that do not see them).  Everything else as in `paged_attention`;
         `batch` needs positions, seg_of_token, cu_seqlens, block_tables and ancestors, and the host need not know how much is cached.  Rows of
         `out` behind the last request's are left as they were.  `out` shares no memory with `q`."""
         raise NotImplementedError

@@ -1,5 +1,5 @@
 """NaN, infinities and the largest numbers in queries, keys and values of a step of drafted trees: what a row sees decides what it is, as the formula says.
-The float32 kernel has that element by element."""
+The float32 kernel has that element by element; on the tensor cores a value that is not finite may reach rows of its request that do not see it."""
 import math
 
 import pytest
@@ -90,8 +90,10 @@ def make(dtype, lens=(70, 30, 0), counts=(20, 7, 40), size=64, seed=1):
 # Of the float32 kernel: one share of the keys; several, of which the joining kernel makes the result; heads of more than 128 elements; of an odd number.
 EXACT = [(F32, (70, 30, 0), (20, 7, 40), 64), (F32, (900, 2003, 5), (20, 7, 40), 64), (F32, (130, 61, 0), (9, 33, 2), 200), (F32, (40, 30, 9), (9, 7, 2), 33),
          (BF, (70, 30, 0), (20, 7, 40), 48), (BF, (900, 303, 5), (20, 7, 40), 200)]
+# Of the tensor cores' kernel: one row tile a request, the same with its keys shared among blocks, pairs of row tiles.
+OTHERS = [(BF, (70, 30, 0), (20, 7, 40), 64), (BF, (9000, 2003, 5), (20, 7, 40), 128), (BF, (900, 300, 5), (90, 140, 70), 64)]
 ids = lambda cases: [f"{'fp32' if t == F32 else 'bf16'}-{a[0]}+{n[0]}-{hd}" for t, a, n, hd in cases]
-BY_SHAPE = pytest.mark.parametrize("dtype,lens,counts,size", EXACT, ids=ids(EXACT))
+BY_SHAPE = pytest.mark.parametrize("dtype,lens,counts,size", EXACT + OTHERS, ids=ids(EXACT + OTHERS))
 BY_EXACT_SHAPE = pytest.mark.parametrize("dtype,lens,counts,size", EXACT, ids=ids(EXACT))
 
 
