@@ -45,8 +45,7 @@ __global__ void __launch_bounds__(256) qk_prepare_kernel(const QkPrepareParams p
                 1.0f / (1.0f + expf(-to_f32(((const T*)p.qkv)[(size_t)t * p.qkv_stride + (size_t)heads_total * hd + h])));
     int page = -1, place = pos % c.page_size;
     if (p.write_cache && !p.q_only && p.slot_map) {
-        const long long slot = p.slot_map[t];
-        if (slot >= 0 && slot < (long long)c.n_pages * c.page_size) { page = (int)(slot / c.page_size); place = (int)(slot % c.page_size); }
+        slot_of(p, c, t, page, place);
     } else if (p.write_cache && !p.q_only) {
         page = b.block_table[(size_t)b.seg_of_token[t] * b.table_width + pos / c.page_size];
         if (page >= c.n_pages) page = -1;                     // the host never lets this happen
@@ -226,8 +225,7 @@ __global__ void __launch_bounds__(256) qk_prepare_vec_kernel(const QkPreparePara
     const int pos = b.positions[t];
     int page = -1, place = pos % c.page_size;
     if (p.write_cache && !p.q_only && p.slot_map) {
-        const long long slot = p.slot_map[t];
-        if (slot >= 0 && slot < (long long)c.n_pages * c.page_size) { page = (int)(slot / c.page_size); place = (int)(slot % c.page_size); }
+        slot_of(p, c, t, page, place);
     } else if (p.write_cache && !p.q_only) {
         const int at = pos / c.page_size;
         page = b.block_table[(size_t)b.seg_of_token[t] * b.table_width + at];
@@ -485,6 +483,7 @@ SPITE_API int spite_qk_prepare(int dtype, const QkPrepareParams* given, const St
     if (p->inv_freq && (p->rotary_dim < 2 || p->rotary_dim % 2 || p->rotary_dim > c->head_dim)) return SPITE_BAD_ARG;
     const int heads = p->num_heads + (p->q_only ? 0 : (p->values_are_keys ? 1 : 2) * c->num_kv_heads);
     if (p->q_only && (p->v_other || p->gates_out || p->values_are_keys)) return SPITE_BAD_ARG;
+    if (p->slot_map && !p->step_tokens) return SPITE_BAD_ARG;
     if (p->values_are_keys && (p->v_other || p->v_inv_freq || p->inv_freq || p->k_gain || c->v_offset != 0 || !c->key_scale))
         return SPITE_BAD_ARG;
     if (p->qkv_stride < (long long)heads * c->head_dim || (p->qkv_stride & 1)) return SPITE_BAD_ARG;

@@ -80,7 +80,15 @@ struct QkPrepareParams {
     // the row of the cache (page * page_size + place in it, or -1: none) that token t's key and value go to, or null: the row of its position (a
     // step of drafted trees, whose nodes lie one behind the other in the cache while their positions are depths)
     const long long* slot_map;
+    // with a slot map: [1], the tokens of the step; the map's rows from there on are left over from other steps and name nothing
+    const int* step_tokens;
 };
+
+// Where token t's key and value go by the slot map: page -1 where they go nowhere.
+__device__ __forceinline__ void slot_of(const QkPrepareParams& p, const PagedCache& c, int t, int& page, int& place) {
+    const long long slot = p.slot_map[t];
+    if (t < *p.step_tokens && slot >= 0 && slot < (long long)c.n_pages * c.page_size) { page = (int)(slot / c.page_size); place = (int)(slot % c.page_size); }
+}
 
 // cos and sin of pos * (freq + low).  With `low` the product's own rounding error and the frequency's are put back to second
 // order, so that the angle of a far position is as exact as that of a near one; without it the float32 product counts.

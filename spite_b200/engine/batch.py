@@ -39,7 +39,8 @@ class StepBatch:
     ancestors: torch.Tensor | None = None   # a step that verifies drafted tokens: [M, words] int32, bit a of row m: token m of its
                                         # request descends from the request's token a (or is it); None: every token follows the one before
     slot_maps: list | None = None       # per group: [M] int64, the cache row (page * page_size + offset) that a token's keys and
-                                        # values go to, -1: none; None: the row of the token's position
+                                        # values go to, -1: none (rows behind the step's last token, by cu_seqlens,
+                                        # write nothing); None: the row of the token's position
     shared: dict = field(default_factory=dict)   # what one layer of the step leaves for a later one (emptied when a
                                                  # forward pass starts)
 

@@ -246,7 +246,7 @@ class KernelSet:
                    value_mix=None, gates_out=None, bias=None, q_only=False, norm_dim=None, value_rotation=None,
                    values_are_keys=False):
         """Encode positions of q and k, normalise, scale q, append k and v to the cache (at the rows that `batch.slot_maps` names, if the
-        step has them, else at their positions).
+        step has them, else at their positions; with slot maps only tokens in front of the last of `batch.cu_seqlens` write).
         `bias` float32 [(nq + 2 nkv) hd]: added to the projection's columns before anything else.  `q_only`: a row of
         qkv holds the q heads alone (and `bias` theirs): the layer reads keys and values that another layer cached.
         qkv [M, >= (nq + 2 nkv) hd] T -> q_out [M, nq hd] T; `cache` is a `LayerCache`.

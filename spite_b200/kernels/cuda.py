@@ -57,7 +57,7 @@ class QkPrepareParams(C.Structure):
                 ("bias", C.c_void_p), ("q_only", C.c_int), ("norm_dim", C.c_int),
                 ("v_inv_freq", C.c_void_p), ("v_rotary_dim", C.c_int), ("v_pairing", C.c_int),
                 ("inv_freq_low", C.c_void_p), ("v_inv_freq_low", C.c_void_p), ("values_are_keys", C.c_int),
-                ("slot_map", C.c_void_p)]
+                ("slot_map", C.c_void_p), ("step_tokens", C.c_void_p)]
 
 
 class AttentionParams(C.Structure):
@@ -1067,7 +1067,10 @@ class CudaKernels(KernelSet):
             slots = self._t(slot_maps[cache.group], torch.int64, "slot_map")
             if slots.numel() < qkv.shape[0]:
                 raise KernelError(f"qk_prepare: the slot map has {slots.numel()} rows for {qkv.shape[0]} tokens")
-            p.slot_map = slots.data_ptr()
+            cu = batch.cu_seqlens
+            if cu is None or not self._t(cu, torch.int32, "cu_seqlens").numel():
+                raise KernelError("qk_prepare: a step with a slot map has cu_seqlens, which say how many of its rows are tokens")
+            p.slot_map, p.step_tokens = slots.data_ptr(), cu.data_ptr() + 4 * (cu.numel() - 1)
         b, c = self._step_tokens(batch, cache.group), self._paged(cache)
         st = self._lib("attention").spite_qk_prepare(self._dt, C.byref(p), C.byref(b), C.byref(c), self._stream())
         self._count("attention", 1)
