@@ -468,40 +468,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 float s[BN];
                 ld64(s, lane_base + sb * BN);
                 const bool open = j0 >= lo_all && j0 + BN <= it.len;      // every key visible to every row
-                if (capped) {
-                    // cap tanh(s scale / cap): the series where every score of the warp's rows is small against the cap, else by 2^x
-                    float big[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int e = 0; e < BN; ++e) big[e & 3] = fmaxf(big[e & 3], fabsf(s[e]));
-                    if (__all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= CAP_SERIES * cap_raw)) {
-                        const f2 inv = pack2(inv_cap_raw, inv_cap_raw), one = pack2(1.f, 1.f), c1 = pack2(CAP_C1, CAP_C1), c2 = pack2(CAP_C2, CAP_C2),
-                                 c3 = pack2(CAP_C3, CAP_C3), c4 = pack2(CAP_C4, CAP_C4), c5 = pack2(CAP_C5, CAP_C5);
-#pragma unroll
-                        for (int e = 0; e < BN; e += 2) {
-                            const f2 v = pack2(s[e], s[e + 1]), t = mul2(v, inv), y = mul2(t, t);
-                            unpack2(mul2(v, fma2(y, fma2(y, fma2(y, fma2(y, fma2(y, c5, c4), c3), c2), c1), one)), s[e], s[e + 1]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < BN; ++e) s[e] = fmaf(-2.f * cap_raw, reciprocal_approx(ex2(s[e] * cap_arg) + 1.f), cap_raw);
-                    }
-                }
-                float tile_bias = 0.f;                           // what the tile's keys have in common of a bias by distance
-                if (biased) {
-                    if (j0 + BN <= it.len) {
-                        tile_bias = slope_raw * (float)(j0 - pos);
-#pragma unroll
-                        for (int e = 0; e < BN; ++e) s[e] = fmaf(slope_raw, (float)e, s[e]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < BN; ++e) {
-                            const int a = j0 + e - it.len;       // (a node sits at its depth, not at its place)
-                            s[e] = fmaf(slope_raw, (float)((a < 0 ? j0 + e : a < it.n ? b.positions[it.first + a] : 0) - pos), s[e]);
-                        }
-                    }
-                }
-                if (!open) {
-                    // 64 bits of what this row sees: settled tokens from its window's end on, then nodes
+                // 64 bits of what this row sees: settled tokens from its window's end on, then nodes
+                auto seen_bits = [&]() {
                     unsigned long long vis = low_bits(it.len - j0) & ~low_bits(lo - j0);
                     if (j0 + BN > it.len) {
                         const int b0 = j0 - it.len;
@@ -522,10 +490,53 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             }
                         vis |= bits;
                     }
-                    if (!row_ok) vis = 0;
+                    return row_ok ? vis : 0ull;
+                };
+                auto keep_seen = [&](unsigned long long vis, float other) {
 #pragma unroll
-                    for (int e = 0; e < BN; ++e) s[e] = ((e < 32 ? (unsigned)vis : (unsigned)(vis >> 32)) >> (e & 31) & 1u) ? s[e] : -INFINITY;
+                    for (int e = 0; e < BN; ++e) s[e] = ((e < 32 ? (unsigned)vis : (unsigned)(vis >> 32)) >> (e & 31) & 1u) ? s[e] : other;
+                };
+                unsigned long long vis = 0;
+                if (CAP && !open) vis = seen_bits();
+                if (capped) {
+                    // cap tanh(s scale / cap): the series where every score that the row sees in the tile is small against the cap, else by 2^x.  Every
+                    // row chooses for itself, so that its bits do not depend on the rows beside it or on keys that it does not see; a warp whose
+                    // rows differ makes both one after the other.  (us, against a choice of the warp: 8 requests of 16 nodes, 8,192 keys, 82.9 / 79.2 with
+                    // a cap of 50, 116 / 95 with one of 3, that about half of the tiles' largest scores reach; all in one loop with a choice by element spills: 92 / 155.)
+                    if (!open) keep_seen(vis, 0.f);
+                    float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < BN; ++e) big[e & 3] = fmaxf(big[e & 3], fabsf(s[e]));
+                    const bool small = !row_ok || fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= CAP_SERIES * cap_raw;
+                    if (small) {
+                        const f2 inv = pack2(inv_cap_raw, inv_cap_raw), one = pack2(1.f, 1.f), c1 = pack2(CAP_C1, CAP_C1), c2 = pack2(CAP_C2, CAP_C2),
+                                 c3 = pack2(CAP_C3, CAP_C3), c4 = pack2(CAP_C4, CAP_C4), c5 = pack2(CAP_C5, CAP_C5);
+#pragma unroll
+                        for (int e = 0; e < BN; e += 2) {
+                            const f2 v = pack2(s[e], s[e + 1]), t = mul2(v, inv), y = mul2(t, t);
+                            unpack2(mul2(v, fma2(y, fma2(y, fma2(y, fma2(y, fma2(y, c5, c4), c3), c2), c1), one)), s[e], s[e + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < BN; ++e) s[e] = fmaf(-2.f * cap_raw, reciprocal_approx(ex2(s[e] * cap_arg) + 1.f), cap_raw);
+                    }
+                    __syncwarp();
                 }
+                float tile_bias = 0.f;                           // what the tile's keys have in common of a bias by distance
+                if (biased) {
+                    if (j0 + BN <= it.len) {
+                        tile_bias = slope_raw * (float)(j0 - pos);
+#pragma unroll
+                        for (int e = 0; e < BN; ++e) s[e] = fmaf(slope_raw, (float)e, s[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < BN; ++e) {
+                            const int a = j0 + e - it.len;       // (a node sits at its depth, not at its place)
+                            s[e] = fmaf(slope_raw, (float)((a < 0 ? j0 + e : a < it.n ? b.positions[it.first + a] : 0) - pos), s[e]);
+                        }
+                    }
+                }
+                if (!open) keep_seen(CAP ? vis : seen_bits(), -INFINITY);
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int e = 0; e < BN; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], s[e]);

@@ -1,0 +1,51 @@
+"""Attention of drafted trees: a row's bits are its own, whatever lies beside it and how often it is asked for."""
+import pytest
+import torch
+
+from draft_helpers import TreeCase
+from spite_b200.cache import Window
+from test_gpu_tree_attention import kernels  # noqa: F401  (the fixture)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+FULL = Window("full")
+
+
+def call(k, case, out=None, **more):
+    q, batch, cache = case.step(DEV)
+    out = torch.zeros_like(q) if out is None else out
+    k.tree_attention(q, out, batch, cache, num_heads=case.heads, window=FULL, softmax_scale=case.size ** -0.5, **more)
+    return out
+
+
+@pytest.mark.parametrize("dtype,heads,size", [(BF, 5, 128), (BF, 5, 64), (BF, 8, 64), (F32, 5, 64)])
+@pytest.mark.parametrize("slopes", [False, True], ids=["cap", "cap and slopes"])
+def test_a_capped_row_depends_on_itself_alone(kernels, dtype, heads, size, slopes):  # noqa: F811
+    """Other rows of its warp (siblings, the next request's, rows that are no node's) and rows of the cache that it does not see change no bit of a row."""
+    k = kernels[dtype]
+    more = dict(score_softcap=4.0)
+    if slopes:
+        more["head_slopes"] = (torch.arange(heads, dtype=F32) / 16).to(DEV)
+    case = TreeCase([200, 70], [9, 30], heads=heads, kv_heads=1, size=size, dtype=dtype, seed=2, padding=True, scale=0.5)
+    case.kv = torch.nan_to_num(case.kv, nan=0.0)              # (padding rows and what lies behind: any numbers)
+    first = call(k, case, **more).clone()
+    assert torch.isfinite(first).all()
+    for _ in range(3):                                       # other launches in between leave other numbers in shared memory
+        call(k, TreeCase([300], [25], heads=heads, kv_heads=1, size=size, dtype=dtype, seed=3, scale=30.0))
+        assert torch.equal(call(k, case, **more), first)
+    keep = case.q.clone()
+    for row in (1, 8, 9, 12):                                # one row louder: all others as before
+        case.q[row] *= 100
+        rest = [i for i in range(case.M) if i != row]
+        assert torch.equal(call(k, case, **more)[rest], first[rest])
+        case.q.copy_(keep)
+    for s in range(2):
+        for j in range(case.lens[s] + case.counts[s], len(case.table[s]) * 64):
+            if int(case.table[s, j // 64]) >= 0:
+                case.kv[:, int(case.table[s, j // 64]), :, j % 64] = 1000.0
+        for i in range(case.counts[s]):
+            if i not in case.sets[s][i]:
+                j = case.lens[s] + i
+                case.kv[:, int(case.table[s, j // 64]), :, j % 64] = -1000.0
+    assert torch.equal(call(k, case, **more), first)
