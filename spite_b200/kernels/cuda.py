@@ -1366,8 +1366,10 @@ class CudaKernels(KernelSet):
             raise KernelError(f"{what}: status and n_free are one number each")
         if not S or not W or not out_width or pages.page_size < 1 or (sets is not None and not n_words):
             raise KernelError(f"{what}: a step needs requests, and pages, tables and sets that are not empty")
+        # (parents without elements have no address, and no address means chains: any other one stands for them, nothing is read there)
+        up = 0 if parents is None else parents.data_ptr() or status.data_ptr()
         call = _LAYOUT_CALL.pack(
-            tables.data_ptr(), held.data_ptr(), _address(free), _address(n_free), slots.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), _address(parents),
+            tables.data_ptr(), held.data_ptr(), _address(free), _address(n_free), slots.data_ptr(), lengths.data_ptr(), new_tokens.data_ptr(), up,
             block.data_ptr(), cu.data_ptr(), positions.data_ptr(), seg.data_ptr(), slot_map.data_ptr(), _address(sets), status.data_ptr(),
             R, W, 0 if free is None else free.numel(), S, out_width, M, 0 if parents is None else parents.numel(), n_words, pages.page_size,
             _WINDOW[pages.window.kind], min(pages.window.size, _MOST))
