@@ -25,7 +25,7 @@ struct LayoutParams {
     const int* slots;            // [n_requests] rows of the step's requests, -1: padding
     const int* lengths;          // [n_rows] tokens cached
     const int* new_tokens;       // [n_requests] tokens that the step brings, -1: the request has ended
-    const int* parents;          // [<= n_tokens] a token's parent within its request (-1: none), or null: every token follows the one before
+    const int* parents;          // [n_parents] a token's parent within its request (-1: none), or null: every token follows the one before
     int* block_table;            // [n_requests, out_width]
     int* cu_seqlens;             // [n_requests + 1]
     int* positions;              // [n_tokens] (as the two below: rows behind the last request's stay as they are)
@@ -503,14 +503,14 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) accept_kernel(const AcceptPara
 
 // Follows every request's tree and moves the accepted rows.  `pieces`: blocks a request.
 SPITE_API int spite_accept_drafts(const AcceptParams* p, int pieces, void* stream) {
-    if (!p || !p->tokens || !p->targets || !p->cu_seqlens || !p->counts || !p->path || !p->emitted) return SPITE_BAD_ARG;
+    if (!p || (p->n_tokens > 0 && (!p->tokens || !p->targets)) || !p->cu_seqlens || !p->counts || !p->path || !p->emitted) return SPITE_BAD_ARG;
     if (p->n_tokens < 0 || p->n_requests < 1 || p->depth < 1 || pieces < 1 || p->n_groups < 0) return SPITE_BAD_ARG;
     if (!p->lengths != !p->lengths_out || (p->lengths && p->n_rows < 1)) return SPITE_BAD_ARG;
     if (p->depth > SPITE_MAX_DRAFTS || p->n_groups > SPITE_ACCEPT_GROUPS || pieces > 65535) return SPITE_UNSUPPORTED;
     uintptr_t bits = 0;
     for (int g = 0; g < p->n_groups; ++g) {
         const AcceptGroup& c = p->groups[g];
-        if (!c.kv || !c.slot_map || c.planes < 1 || c.caches < 1 || c.n_pages < 1 || c.num_kv_heads < 1 || c.page_size < 1 || c.row_bytes < 1)
+        if (!c.kv || (p->n_tokens > 0 && !c.slot_map) || c.planes < 1 || c.caches < 1 || c.n_pages < 1 || c.num_kv_heads < 1 || c.page_size < 1 || c.row_bytes < 1)
             return SPITE_BAD_ARG;
         bits |= (uintptr_t)c.kv | (uintptr_t)c.plane_bytes | (uintptr_t)c.row_bytes;
     }

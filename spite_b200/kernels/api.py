@@ -318,7 +318,8 @@ class KernelSet:
     def accept_drafts(self, tokens, parents, targets, cu_seqlens, caches, *, counts, path, emitted, slots=None, lengths=None, lengths_out=None):
         """Follows every request's tree (tokens, parents as in `layout_step`, None: chains; int32 [M]) by what the model says: from node 0 to the
         lowest-numbered child that is the node's target (targets, int32 [M]), and on.  counts [S] int32: nodes on the way (0 for a request without
-        tokens), path [S, D] int32 their numbers, emitted [S, D] their targets, -1 behind the last; a way ends after D nodes.  The rows
+        tokens), path [S, D] int32 their numbers, emitted [S, D] their targets, -1 behind the last; a way ends after D nodes, and in front of a node
+        numbered 1,024 or more.  The rows
         of the way's nodes move to the places that follow the request's cached tokens: in every cache of `caches`, a list of (kv [caches, planes,
         pages, kv heads, page_size, head_dim], slot_map [M] int64, key_scales [caches, pages, kv heads, page_size] float32 or None), the row of
         slot_map[node] goes to slot_map[number on the way] (no row where either is negative).  With `lengths` (int32 [rows], and `lengths_out`, which may
