@@ -501,7 +501,8 @@ int launch(const TreeCall& a, float* partial, int n_splits, int share_keys, cuda
     if ((long long)c.num_kv_heads * chunks > 65535) return SPITE_UNSUPPORTED;
     const dim3 grid(a.b.n_tokens / nodes + a.x.n_segments, c.num_kv_heads * chunks, n_splits);       // (no request has a chunk more than fill it)
     auto k = async ? attn_tree_kernel<T, HD4, true> : attn_tree_kernel<T, HD4, false>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SPITE_LAUNCH_FAILED;
+    static std::atomic<unsigned long long> done[2];
+    if (!allow_shared(k, smem_bytes<T, 64 / HD4>(128 * HD4), done[async])) return SPITE_LAUNCH_FAILED;
     SPITE_LAUNCH(k, grid, THREADS, smem, st, p, a.b, c, a.x, partial, nodes, n_splits, (share_keys + 64 / HD4 - 1) / (64 / HD4));
     if (n_splits > 1)
         SPITE_LAUNCH((attn_tree_join_kernel<T, HD4>), dim3(a.b.n_tokens, (p.num_heads + 3) / 4), JOIN_THREADS, 0, st, p, a.x, (const float*)partial, hd, n_splits);

@@ -8,6 +8,8 @@
 #pragma once
 #include "attention.cuh"
 
+#include <atomic>
+
 struct TreeStep {
     const int* cu_seqlens;       // [n_segments + 1]
     const unsigned* ancestors;   // [tokens, n_words]
@@ -27,6 +29,19 @@ static inline bool tree_call_ok(const TreeCall& a) {
     if (a.b.n_tokens < 0 || a.b.table_width < 1 || a.c.n_pages < 1 || a.c.page_size < 1 || a.x.n_segments < 1 || a.x.n_words < 1) return false;
     if (a.p.num_heads < 1 || a.c.num_kv_heads < 1 || a.p.num_heads % a.c.num_kv_heads || a.c.head_dim < 1) return false;
     return a.p.window_kind >= 0 && a.p.window_kind <= 2 && (a.p.window_kind == SPITE_WINDOW_FULL || a.p.window_size >= 1) && distance_bias_ok(&a.p);
+}
+
+// Lets a kernel take `most` bytes of dynamic shared memory, the most that any call of it needs: once a device (`done` has a bit each), since the limit
+// is the process's, and a call that set it to its own size could lower it under another thread's launch.
+template <typename K>
+static bool allow_shared(K kernel, size_t most, std::atomic<unsigned long long>& done) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return false;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_release);
+    return true;
 }
 
 // Is node `i` of the segment that starts at token `first` a token of its own (its own bit is set)?

@@ -730,9 +730,12 @@ int launch(const AttentionParams& p, const StepTokens& b, const PagedCache& c, c
         if (!make_map(&mk, c.kv, 2, dims, strides, box)) return SPITE_LAUNCH_FAILED;
         if (!make_map(&mv, (const __nv_bfloat16*)c.kv + c.v_offset, 2, dims, strides, box)) return SPITE_LAUNCH_FAILED;
     }
-    const size_t smem = (2 * (size_t)NKB * BM + stages(NKB) * (size_t)NKB * BN) * 128 + (size_t)(x.n_segments < MAX_SEGMENTS ? x.n_segments : MAX_SEGMENTS) * 20 + 4;
-    auto k = p.head_slopes ? attn_tree_tc_kernel<NKB, FORM_ANY> : p.score_softcap > 0.f ? attn_tree_tc_kernel<NKB, FORM_CAP> : attn_tree_tc_kernel<NKB, FORM_PLAIN>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SPITE_LAUNCH_FAILED;
+    auto smem_for = [](int segments) { return (2 * (size_t)NKB * BM + stages(NKB) * (size_t)NKB * BN) * 128 + (size_t)segments * 20 + 4; };
+    const size_t smem = smem_for(x.n_segments < MAX_SEGMENTS ? x.n_segments : MAX_SEGMENTS);
+    const int form = p.head_slopes ? FORM_ANY : p.score_softcap > 0.f ? FORM_CAP : FORM_PLAIN;
+    auto k = form == FORM_ANY ? attn_tree_tc_kernel<NKB, FORM_ANY> : form == FORM_CAP ? attn_tree_tc_kernel<NKB, FORM_CAP> : attn_tree_tc_kernel<NKB, FORM_PLAIN>;
+    static std::atomic<unsigned long long> done[3];
+    if (!allow_shared(k, smem_for(MAX_SEGMENTS), done[form])) return SPITE_LAUNCH_FAILED;
     const long long tiles = (long long)b.table_width * c.page_size / BN;
     for (int s0 = 0; s0 < x.n_segments; s0 += MAX_SEGMENTS) {
         TreeStep some = x;

@@ -1,4 +1,6 @@
-"""Attention of drafted trees: a row's bits are its own, whatever lies beside it and how often it is asked for."""
+"""Attention of drafted trees: a row's bits are its own, whatever lies beside it and how often it is asked for, and whatever other host threads call."""
+import threading
+
 import pytest
 import torch
 
@@ -49,3 +51,39 @@ def test_a_capped_row_depends_on_itself_alone(kernels, dtype, heads, size, slope
                 j = case.lens[s] + i
                 case.kv[:, int(case.table[s, j // 64]), :, j % 64] = -1000.0
     assert torch.equal(call(k, case, **more), first)
+
+
+@pytest.mark.parametrize("dtype,shapes", [(BF, [(600, 64, 64), (1, 64, 64)]), (F32, [(2, 200, 64), (2, 136, 64)]), (F32, [(2, 128, 64), (2, 16, 64)])],
+                         ids=["requests", "large heads", "small heads"])
+def test_two_host_threads(dtype, shapes):
+    """Calls of different sizes from two threads, each with kernels and a stream of its own: a launch's shared memory is not limited by another's."""
+    from spite_b200.kernels.cuda import CudaKernels
+    errors, results = [], [None, None]
+    cases = [TreeCase([9] * n, [2] * n, heads=2, kv_heads=1, size=size, page=page, dtype=dtype, seed=n + size) for n, size, page in shapes]
+    ks = [CudaKernels(dtype, DEV) for _ in cases]
+    want = [call(k, c).clone() for k, c in zip(ks, cases)]
+    torch.cuda.synchronize()
+    start = threading.Barrier(2)
+
+    def work(i):
+        try:
+            q, batch, cache = cases[i].step(DEV)
+            out = torch.zeros_like(q)
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.default_stream())
+            start.wait(timeout=60)
+            with torch.cuda.stream(stream):
+                for _ in range(3000):
+                    ks[i].tree_attention(q, out, batch, cache, num_heads=2, window=FULL, softmax_scale=cases[i].size ** -0.5)
+            stream.synchronize()
+            results[i] = out
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for got, right in zip(results, want):
+        assert torch.equal(got, right)
