@@ -737,6 +737,7 @@ int launch(const AttentionParams& p, const StepTokens& b, const PagedCache& c, c
     static std::atomic<unsigned long long> done[3];
     if (!allow_shared(k, smem_for(MAX_SEGMENTS), done[form])) return SPITE_LAUNCH_FAILED;
     const long long tiles = (long long)b.table_width * c.page_size / BN;
+    int launches = 0;
     for (int s0 = 0; s0 < x.n_segments; s0 += MAX_SEGMENTS) {
         TreeStep some = x;
         StepTokens tokens = b;
@@ -744,15 +745,20 @@ int launch(const AttentionParams& p, const StepTokens& b, const PagedCache& c, c
         some.n_segments = x.n_segments - s0 < MAX_SEGMENTS ? x.n_segments - s0 : MAX_SEGMENTS;
         tokens.block_table += (size_t)s0 * b.table_width;
         SPITE_LAUNCH(k, n_sm, THREADS, smem, st, mq, mk, mv, p, tokens, c, some, tpt, box_tokens, cut, s_waits);
-        if (tiles >= 2 * PIECE)                                  // (with fewer no item is cut)
+        ++launches;
+        if (tiles >= 2 * PIECE) {                                // (with fewer no item is cut)
             SPITE_LAUNCH(attn_tree_tc_join_kernel, dim3(n_sm, hd / JOIN_COLS, 2), BM, 0, st, p, cut, nkv, tpt, hd);
+            ++launches;
+        }
     }
-    return spite_launch_status();
+    const int status = spite_launch_status();
+    return status == SPITE_OK ? launches : status;
 }
 
 }  // namespace
 
-// `n_sm`: number of multiprocessors (a block each).  `scratch`: n_sm * (4 * (head_dim + 2) * 128 + 4) floats.
+// `n_sm`: number of multiprocessors (a block each).  `scratch`: n_sm * (4 * (head_dim + 2) * 128 + 4) floats.  Returns the number of launches,
+// or what is wrong.
 SPITE_API int spite_tree_attention_tc(const TreeCall* call, int n_sm, float* scratch, long long n_floats, void* stream) {
     if (!call || !scratch || n_sm < 1 || !tree_call_ok(*call)) return SPITE_BAD_ARG;
     const AttentionParams& p = call->p;

@@ -1327,8 +1327,8 @@ class CudaKernels(KernelSet):
             st = self._entry("attention_tree_tc", "spite_tree_attention_tc")(
                 call, self.sm_count, part.data_ptr(), n_floats, stream)
             if st != -2:                        # -2: more than 128 heads a kv head, a tensor that does not start at 16 bytes, sizes beyond 32 bits
-                self._count("attention_tree_tc", 2)
-                _check(st, f"{what} (tcgen05)")
+                _check(min(st, 0), f"{what} (tcgen05)")
+                self._count("attention_tree_tc", st)
                 return
         # The float32 kernel: blocks of 32 rows and shares of the keys, of 128 or as many more as keep the blocks of full tables at eight a
         # multiprocessor (two run at once; requests are shorter than their tables, and the blocks of shares they do not have leave at once).

@@ -53,6 +53,19 @@ def test_a_capped_row_depends_on_itself_alone(kernels, dtype, heads, size, slope
     assert torch.equal(call(k, case, **more), first)
 
 
+def test_launches_are_counted(kernels):  # noqa: F811
+    k = kernels[BF]
+
+    def launches(lens, counts, width=None):
+        before = k.launches_by_library["attention_tree_tc"]
+        call(k, TreeCase(lens, counts, heads=4, kv_heads=1, size=64, dtype=BF, width=width))
+        return k.launches_by_library["attention_tree_tc"] - before
+    assert launches([100], [8]) == 1                          # (two pages: nothing is shared, nothing is joined)
+    assert launches([1000], [8]) == 2
+    assert launches([10] * 641, [1] * 641) == 2               # (640 requests a launch)
+    assert launches([10] * 641, [1] * 641, width=20) == 4
+
+
 @pytest.mark.parametrize("dtype,shapes", [(BF, [(600, 64, 64), (1, 64, 64)]), (F32, [(2, 200, 64), (2, 136, 64)]), (F32, [(2, 128, 64), (2, 16, 64)])],
                          ids=["requests", "large heads", "small heads"])
 def test_two_host_threads(dtype, shapes):
