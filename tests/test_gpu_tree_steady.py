@@ -6,7 +6,7 @@ import torch
 
 from draft_helpers import TreeCase
 from spite_b200.cache import Window
-from test_gpu_tree_attention import kernels  # noqa: F401  (the fixture)
+from test_gpu_tree_attention import kernels, run  # noqa: F401  (the fixture)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -51,6 +51,30 @@ def test_a_capped_row_depends_on_itself_alone(kernels, dtype, heads, size, slope
                 j = case.lens[s] + i
                 case.kv[:, int(case.table[s, j // 64]), :, j % 64] = -1000.0
     assert torch.equal(call(k, case, **more), first)
+
+
+@pytest.mark.parametrize("dtype,heads,size", [(BF, 8, 128), (BF, 4, 64), (F32, 4, 64)])
+def test_requests_of_several_launches_with_shared_items(kernels, dtype, heads, size):  # noqa: F811
+    """1,500 requests (640 a launch), long ones in every launch, whose keys are shared among blocks: the launches use one scratch one after the other."""
+    lens = [5000 if s in (3, 700, 1290) else 9000 if s in (639, 640, 1499) else s % 3 for s in range(1500)]
+    counts = [20 if n > 100 else s % 2 for s, n in enumerate(lens)]
+    case = TreeCase(lens, counts, heads=heads, kv_heads=1, size=size, dtype=dtype, seed=8)
+    out = run(kernels, case)
+    for _ in range(3):
+        assert torch.equal(call(kernels[dtype], case), out)
+
+
+def test_launches_are_counted(kernels):  # noqa: F811
+    k = kernels[BF]
+
+    def launches(case):
+        before = k.launches_by_library["attention_tree_tc"]
+        call(k, case)
+        return k.launches_by_library["attention_tree_tc"] - before
+    assert launches(TreeCase([100], [8], heads=4, kv_heads=1, size=64, dtype=BF)) == 1           # (two pages: nothing is shared)
+    assert launches(TreeCase([1000], [8], heads=4, kv_heads=1, size=64, dtype=BF)) == 2
+    assert launches(TreeCase([10] * 641, [1] * 641, heads=4, kv_heads=1, size=64, dtype=BF)) == 2
+    assert launches(TreeCase([10] * 640 + [1000], [1] * 641, heads=4, kv_heads=1, size=64, dtype=BF)) == 4
 
 
 def test_launches_are_counted(kernels):  # noqa: F811
