@@ -14,8 +14,8 @@
 // of the cache that are no visible token's are read as zeros, so they may hold anything.
 //
 // NaN, infinities and numbers next to the largest cannot be split; and the products would carry a value that is not finite into rows that do not see
-// it, 0 x NaN being NaN.  Where a tile has such a number, the warps that meet it make their products again one by one in float32, with a row's own
-// keys alone.  Looking for them takes 1 to 3 % (8 requests of 16 nodes, 2,048 keys, 40 heads on 8 of 128: 271 us, 265 without).
+// it, 0 x NaN being NaN.  Where a warp meets such a number, the results that it goes into are made again one by one in float32, with a row's own
+// keys alone; all others keep their bits.  Looking for them takes 1 to 3 % (8 requests of 16 nodes, 2,048 keys, 40 heads on 8 of 128: 273 us, 265 without).
 //
 // Score, mask and softmax: crates/spite-compute/src/flash_attn.rs:111-156, with the mask of attention_tree.cuh.
 #include "attention_tree.cuh"
@@ -51,17 +51,27 @@ __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], const
 }
 // What a row weighs a key with that it does not see: zero, and by its sign apart from a weight that has become zero.
 constexpr float UNSEEN = -0.f;
-// A query's product with a key, and a row's sum over a column of the values that it sees (`weights` P_STRIDE apart, `column` `stride`), in float32.
-template <typename T> __device__ __noinline__ float product(const float* q, const T* k, int n) {
+// A query's product with a key, and a row's sum over a column of the values that it sees (`weights` P_STRIDE apart, `column` `stride`), in float32, where
+// a number among them cannot be split; where all can, what the products have `made`.
+template <typename T> __device__ __noinline__ float product(const float* q, const T* k, int n, float made) {
     float sum = 0.f;
-    for (int d = 0; d < n; ++d) sum = fmaf(q[d], to_f32(k[d]), sum);
-    return sum;
+    bool all = true;
+    for (int d = 0; d < n; ++d) {
+        const float a = q[d], b = to_f32(k[d]);
+        all &= splits(a) && splits(b);
+        sum = fmaf(a, b, sum);
+    }
+    return all ? made : sum;
 }
-template <typename T> __device__ __noinline__ float seen_values(const float* weights, const T* column, int stride, int n) {
+template <typename T> __device__ __noinline__ float seen_values(const float* weights, const T* column, int stride, int n, float made) {
     float sum = 0.f;
-    for (int j = 0; j < n; ++j)
-        if (__float_as_uint(weights[j * P_STRIDE]) != __float_as_uint(UNSEEN)) sum = fmaf(weights[j * P_STRIDE], to_f32(column[j * stride]), sum);
-    return sum;
+    bool all = true;
+    for (int j = 0; j < n; ++j) {
+        const float w = weights[j * P_STRIDE], v = to_f32(column[j * stride]);
+        all &= splits(w) && splits(v);
+        if (__float_as_uint(w) != __float_as_uint(UNSEEN)) sum = fmaf(w, v, sum);
+    }
+    return all ? made : sum;
 }
 // 16 bytes from global to shared memory, or zeros.
 __device__ __forceinline__ void copy16(void* to, const void* from, bool there) {
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                 for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        s[k][e] = product(q_s + (16 * half + g + 8 * (e >> 1)) * q_stride, k_s + (quarter * 8 * KT + 8 * k + 2 * cc + (e & 1)) * k_stride, hd);
+                        s[k][e] = product(q_s + (16 * half + g + 8 * (e >> 1)) * q_stride, k_s + (quarter * 8 * KT + 8 * k + 2 * cc + (e & 1)) * k_stride, hd, s[k][e]);
             }
             const int j0 = lo_any + ti * BN;
             if (plain && j0 >= lo_all && j0 + BN <= len) {     // settled keys that every row sees
@@ -388,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tree_kernel(const AttentionPa
                     if (quarter * 32 * HD4 + 8 * e >= hd8) continue;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        part[e][k] = seen_values(p_s + 16 * half + g + 8 * (k >> 1), v_s + quarter * 32 * HD4 + 8 * e + 2 * cc + (k & 1), v_stride, BN);
+                        part[e][k] = seen_values(p_s + 16 * half + g + 8 * (k >> 1), v_s + quarter * 32 * HD4 + 8 * e + 2 * cc + (k & 1), v_stride, BN, part[e][k]);
                 }
             }
 #pragma unroll

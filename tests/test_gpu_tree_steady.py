@@ -53,6 +53,28 @@ def test_a_capped_row_depends_on_itself_alone(kernels, dtype, heads, size, slope
     assert torch.equal(call(k, case, **more), first)
 
 
+@pytest.mark.parametrize("dtype,size", [(BF, 128), (BF, 48), (F32, 64), (F32, 200)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_what_is_not_finite_changes_no_other_row(kernels, dtype, size, value):  # noqa: F811
+    """A query, or a drafted node's key, that is not finite: rows that do not see it keep their bits."""
+    k = kernels[dtype]
+    case = TreeCase([300, 70], [9, 30], heads=4, kv_heads=2, size=size, dtype=dtype, seed=2, trees=[[-1, 0, 0, 1, 2, 3, 3, 4, 4], list(range(-1, 29))])
+    first = call(k, case).clone()
+    assert torch.isfinite(first).all()
+    for row in (0, 5, 20):
+        keep = case.q[row].clone()
+        case.q[row, 7] = value
+        rest = [i for i in range(case.M) if i != row]
+        got = call(k, case)
+        assert torch.equal(got[rest], first[rest]) and not torch.isfinite(got[row]).all()
+        case.q[row] = keep
+    j = 300 + 1                                              # node 1 of the first tree, seen by 1, 3, 5 and 6
+    case.kv[0, int(case.table[0, j // 64]), :, j % 64, 5] = float("nan")
+    got = call(k, case)
+    rest = [i for i in range(case.M) if i not in (1, 3, 5, 6)]
+    assert torch.equal(got[rest], first[rest]) and torch.isnan(got[[1, 3, 5, 6]]).all()
+
+
 @pytest.mark.parametrize("dtype,heads,size", [(BF, 8, 128), (BF, 4, 64), (F32, 4, 64)])
 def test_requests_of_several_launches_with_shared_items(kernels, dtype, heads, size):  # noqa: F811
     """1,500 requests (640 a launch), long ones in every launch, whose keys are shared among blocks: the launches use one scratch one after the other."""
