@@ -8,14 +8,14 @@
 // which leaves out 2^-22 of a product at most (rest x rest, and the rest's own rounding), less than float32 sums over a head round off;
 // stored bfloat16 has no rest.  On the multiply-add units the reads of shared memory bound the kernel: 16 bytes a lane take four cycles whether
 // lanes read the same or not, and 32 rows leave no room for tiles large enough to use a word often (one float32 request of 4 x 13 nodes, 2,047
-// keys, 16 heads on 4 of 128: 66 us that way, 36 now, 33 of them this kernel).  What bounds it now is latency, of the few tiles a block works on and of
-// finding them (tensor pipe 20 % busy, 0.48 instructions a cycle and scheduler).  The softmax is kept
+// keys, 16 heads on 4 of 128: 66 us that way, 37 now, 34 of them this kernel).  What bounds it now is latency, of the few tiles a block works on and of
+// finding them (tensor pipe 20 % busy, 0.50 instructions a cycle and scheduler).  The softmax is kept
 // as a running maximum and sum; shares of the keys leave their unnormalised results, which a second kernel adds up in the order of the keys.  The rows
 // of the cache that are no visible token's are read as zeros, so they may hold anything.
 //
 // NaN, infinities and numbers next to the largest cannot be split; and the products would carry a value that is not finite into rows that do not see
 // it, 0 x NaN being NaN.  Where a warp meets such a number, the results that it goes into are made again one by one in float32, with a row's own
-// keys alone; all others keep their bits.  Looking for them takes 1 to 3 % (8 requests of 16 nodes, 2,048 keys, 40 heads on 8 of 128: 273 us, 265 without).
+// keys alone; all others keep their bits.  Looking for them takes 2 to 4 % (8 requests of 16 nodes, 2,048 keys, 40 heads on 8 of 128: 273 us, 265 without).
 //
 // Score, mask and softmax: crates/spite-compute/src/flash_attn.rs:111-156, with the mask of attention_tree.cuh.
 #include "attention_tree.cuh"

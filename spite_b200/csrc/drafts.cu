@@ -3,9 +3,11 @@
 // the walk down every request's tree by the target tokens with the accepted tokens' cache rows moved to their places.
 //
 // Both are bound by latency: a few dependent rounds through L2 and what is launched around them.  us on the device, in a graph of calls (a call
-// takes the host 11 to 12): the layout of one request 5.2, of 64 trees with tables of 2,049 pages 8.6, of 250 portions with a sliding window 7.5; accepted
-// paths of one request 4.2, of 8 requests in 48 caches 5.1, of 61 in 24 caches, 25.8 MB read and written, 8.6 (3.0 TB/s, much of it in L2).
-// What bounds the layout is the plan, some ten dependent rounds by one block (L2, block barriers, the scan); what bounds the accepted paths is the
+// takes the host 11 to 12): the layout of one request 5.4, of 64 trees with tables of 2,049 pages 8.4 where no page moves and 28 where two ended
+// requests give 1,659 pages back and 16 are taken, of 250 portions with a sliding window 7.6, with 221 pages back and 32 taken 13.7; accepted
+// paths of one request 4.1, of 8 requests in 48 caches 5.1, of 61 in 24 caches, 25.8 MB read and written, 8.5 (3.0 TB/s, much of it in L2).
+// What bounds the layout is the plan, some ten dependent rounds by one block (L2, block barriers, the scan), and the pages that go back, a warp
+// a request; what bounds the accepted paths is the
 // chain lengths -> tree -> slot map -> rows, four round trips, and the largest only in part the bytes.
 #include "common.cuh"
 

@@ -211,7 +211,8 @@ class Engine:
         node, int32 [nodes] (default: the argmax, as in greedy decoding).  From node 0 the way goes to the child that is its node's target, as far
         as there is one.  Returns for every request the targets along its way, which are the next tokens that single steps would have produced (as many as
         nodes on the way, at least one); all of them but the last are cached then, like the tree's root, and the last is the next step's first
-        token.  The other nodes leave nothing behind.  Nothing is changed if the step cannot run."""
+        token.  The other nodes leave nothing behind.  Every node takes a place of the cache while the step runs: cached tokens and nodes together
+        are limited by `max_positions`.  Nothing is changed if the step cannot run."""
         trees = [t if isinstance(t, DraftTree) else DraftTree(*t) for t in trees]
         self.check()
         if not all(part.follows_trees for _, part in self.model.parts() if isinstance(part, Mixer)):
